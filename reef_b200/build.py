@@ -22,7 +22,7 @@ INCLUDE = os.path.join(ROOT, "include")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static",
+    "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static", "--threads", "0",
 ]
 CXX_FLAGS = ["-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-pthread", "-Wall"]
 # REEF_DEBUG_AIDS=1 in the environment builds the development flavour: phase-trace stamps in the tensor-core kernel,

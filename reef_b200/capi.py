@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 
 import numpy as np
 
@@ -153,6 +154,50 @@ def launch_count() -> int:
 
 def _buf(a: np.ndarray):
     return C.c_void_p(a.ctypes.data)
+
+
+class Kernel:
+    """One kernel of the registry on device pointers (``reef_module_get_kernel`` / ``reef_launch``): for programs that hold their own
+    device memory.  Resolving a name needs no GPU.  ``prepare`` does a device's one-time work and has to run ahead of the first launch
+    there, outside a stream capture; launches are asynchronous and may be captured."""
+
+    _module, _lock = None, threading.Lock()
+
+    def __init__(self, name: str):
+        self._lib = lib = cuda_lib()
+        self.name, self._h = name, C.c_void_p()
+        with Kernel._lock:      # a module is a list of its kernels
+            if Kernel._module is None:
+                module = C.c_void_p()
+                _check(lib.reef_module_open(None, C.byref(module)), "reef_module_open")
+                lib.reef_launch.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]
+                Kernel._module = module
+            _check(lib.reef_module_get_kernel(Kernel._module, name.encode(), C.byref(self._h)), f"reef_module_get_kernel({name})")
+        self._dims, smem, nargs = (C.c_uint32 * 6)(), C.c_uint32(), C.c_int()
+        _check(lib.reef_kernel_geometry(self._h, self._dims, C.byref(smem), C.byref(nargs)), "reef_kernel_geometry")
+        self._smem, self.num_args = smem.value, nargs.value
+        self._words, self._pointers = C.c_uint64 * nargs.value, C.c_void_p * nargs.value
+        need = (C.c_size_t * max(16, nargs.value))()
+        _check(lib.reef_kernel_arg_bytes(self._h, need, C.c_int(len(need))), "reef_kernel_arg_bytes")
+        self.arg_bytes = list(need)[:nargs.value]
+
+    def _args(self, pointers):
+        if len(pointers) != self.num_args:
+            raise ReefError(OUT_OF_RANGE, self.name, f"{self.num_args} arguments, got {len(pointers)}")
+        words = self._words(*pointers)
+        at = C.addressof(words)
+        return words, self._pointers(*range(at, at + 8 * len(pointers), 8))
+
+    def prepare(self, pointers):
+        words, args = self._args(pointers)
+        _check(self._lib.reef_kernel_prepare(self._h, args), f"reef_kernel_prepare({self.name})")
+
+    def launch(self, pointers, stream: int = 0):
+        """``pointers``: device addresses, positional; ``stream``: a cudaStream_t of the current device."""
+        words, args = self._args(pointers)
+        rc = self._lib.reef_launch(self._h, self._dims, self._smem, stream, args)
+        if rc != SUCC:
+            _check(rc, f"reef_launch({self.name})")
 
 
 class HybridExecutor:

@@ -14,9 +14,11 @@
 #include <string>
 
 #include "attention_tc.cuh"
+#include "beam.cuh"
 #include "bert.cuh"
 #include "conv_simt.cuh"
 #include "conv_tc_params.h"
+#include "paged_attention.cuh"
 #include "simple.cuh"
 
 namespace reef {
@@ -37,7 +39,8 @@ struct TcCache {
     bool valid = false;
 };
 
-static inline bool is_tc_family(int f) { return f == F_CONV_TC || f == F_ATTENTION_TC; }
+// families with a kernel of their own, launched beside the dispatcher and not inside it
+static inline bool is_own_family(int f) { return f == F_CONV_TC || f == F_ATTENTION_TC || f == F_PAGED_ATTENTION; }
 
 static thread_local std::string g_err;
 void set_error(const std::string& s) { g_err = s; }
@@ -95,6 +98,143 @@ static void plan_conv_simt(KernelSpec* s) {
     p.tiles_c = ceil_div(p.co, w.tc);
     s->task.nblocks = p.tiles_p * p.tiles_c;
     s->dyn_smem = kConvSimtSmem;
+}
+
+// Operators of a decoding step: attributes that are out of range make the name unknown, so that no launch ever sees them.
+static bool need_between(const Attrs& a, const char* k, long long lo, long long hi, int* out) {
+    const long long v = a.get(k, lo - 1);
+    if (v < lo || v > hi) return false;
+    *out = (int)v;
+    return true;
+}
+
+// one that may be absent
+static bool maybe_between(const Attrs& a, const char* k, long long lo, long long hi, int absent, int* out) {
+    *out = absent;
+    return !a.has(k) || need_between(a, k, lo, hi, out);
+}
+
+static bool paged_pages(const Attrs& a, PagedP* p) {
+    if (!need_between(a, "ps", 1, 1024, &p->ps) || !need_between(a, "pages", 1, 0x7fffffff, &p->pages)) return false;
+    if ((long long)p->pages * p->ps > 0x7fffffffLL) return false;       // a token's slot is an int
+    while ((1 << p->ps_shift) < p->ps) p->ps_shift++;
+    p->ps_mul = (unsigned)((1ull << (31 + p->ps_shift)) / p->ps) + 1;
+    return true;
+}
+
+static bool paged_heads(const Attrs& a, PagedP* p) {
+    if (!need_between(a, "kvh", 1, 1024, &p->kvh) || !need_between(a, "d", 64, 256, &p->d) || (p->d & (p->d - 1))) return false;
+    return maybe_between(a, "kt", KT_FP32, KT_FP16, KT_FP32, &p->kt);
+}
+
+static double cache_bytes(int kt) { return kt == KT_FP32 ? 4.0 : 2.0; }
+
+static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
+    KTask& t = s->task;
+    PagedP& p = t.p.paged;
+    if (op == "reef_page_tables") {
+        if (!need_between(a, "rows", 1, kTablesMaxRows, &p.rows) || !need_between(a, "tokens", 1, 1 << 20, &p.tokens) || !paged_pages(a, &p) ||
+            p.pages > kTablesMaxPages || !need_between(a, "mp", 1, (1 << 30) / p.ps, &p.mp) || (long long)p.rows * p.mp > (1 << 30))
+            return false;
+        p.has_fork = a.get("fork", 0) != 0;
+        // Rows are written by up to 32 blocks, 4096 ids to a block; what comes before is done by each of them.
+        p.split = (int)std::min<long long>(std::min(32, p.rows), ((long long)p.rows * p.mp + 4095) / 4096);
+        t.family = F_PAGE_TABLES;
+        t.nblocks = p.split;
+        s->dyn_smem = (uint32_t)tables_smem(p.rows, p.pages);
+        s->nargs = p.has_fork ? 10 : 8;
+        s->bytes = 4.0 * (2.0 * p.rows * p.mp + 4.0 * p.tokens + (p.has_fork ? 10.0 : 5.0) * p.rows);
+        return true;
+    }
+    if (op == "reef_paged_append") {
+        if (!need_between(a, "tokens", 1, 1 << 20, &p.tokens) || !paged_pages(a, &p) || !paged_heads(a, &p)) return false;
+        const int row = p.kvh * p.d;
+        if (!maybe_between(a, "forks", 0, 1 << 20, 0, &p.rows)) return false;
+        p.has_fork = p.rows > 0;
+        // row strides and offsets in floats: keys and values of a fused projection lie side by side
+        if (!maybe_between(a, "ks", 0, 0x7fffffff, row, &p.qs) || !maybe_between(a, "vs", 0, 0x7fffffff, row, &p.vs) ||
+            !maybe_between(a, "ko", 0, 0x7fffffff, 0, &p.qo) || !maybe_between(a, "vo", 0, 0x7fffffff, 0, &p.vo))
+            return false;
+        if ((p.qs | p.vs | p.qo | p.vo) & 3 || (p.tokens > 1 && (p.qs < row || p.vs < row))) return false;
+        if ((long long)p.rows * p.kvh > (1 << 30)) return false;
+        p.split = append_token_blocks(p);
+        t.family = F_PAGED_APPEND;
+        t.nblocks = p.split + append_fork_blocks(p);
+        s->nargs = p.has_fork ? 6 : 5;
+        s->bytes = 2.0 * p.tokens * row * (4.0 + cache_bytes(p.kt)) + 16.0 * (p.tokens + p.rows);
+        return true;
+    }
+    // attention, with and without parts, and the join
+    if (!need_between(a, "tokens", 1, 1 << 16, &p.tokens) || !need_between(a, "heads", 1, 1024, &p.heads) || !paged_heads(a, &p) || p.heads % p.kvh)
+        return false;
+    const int group = p.heads / p.kvh;
+    p.subs = ceil_div(group, paged_gb_max(p.kt, p.d));
+    p.gb = ceil_div(group, p.subs);
+    if (p.gb > 2) p.gb = 4;
+    if ((long long)p.tokens * p.kvh * p.subs > (1 << 30)) return false;
+    const bool parts = op == "reef_paged_attention_parts", join = op == "reef_paged_attention_join";
+    if (!need_between(a, "rows", 1, 1 << 16, &p.rows) || !paged_pages(a, &p) || !need_between(a, "mp", 1, (1 << 30) / p.ps, &p.mp)) return false;
+    const long long passes = (long long)p.tokens * p.kvh * p.subs;
+    const int units = ceil_div(p.mp * p.ps, paged_unit(p));
+    // With parts: two blocks to an SM, fewer where the longest rows would not give every warp its least work.
+    const int blocks = (int)std::min<long long>(2 * kSmsPlanned, (passes * units + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits));
+    if (join) {
+        p.split = blocks;
+        t.family = F_PAGED_JOIN;
+        t.nblocks = blocks * p.gb;
+        s->dyn_smem = (uint32_t)paged_join_smem(p.d);
+        s->nargs = 2;
+        s->bytes = (double)paged_parts_bytes(p, blocks);
+        return true;
+    }
+    if (!maybe_between(a, "qs", 0, 0x7fffffff, p.heads * p.d, &p.qs) || !maybe_between(a, "qo", 0, 0x7fffffff, 0, &p.qo)) return false;
+    if ((p.qs | p.qo) & 3 || (p.tokens > 1 && p.qs < p.heads * p.d)) return false;
+    t.family = F_PAGED_ATTENTION;
+    s->tensor_core = 1;     // launched on its own, a block to half an SM
+    s->dyn_smem = (uint32_t)paged_attention_smem(p);
+    // the most that a launch can have to do: every row as long as its table
+    s->flops = 4.0 * p.tokens * (double)p.heads * p.d * p.mp * p.ps;
+    s->bytes = 2.0 * std::min((double)p.tokens * p.mp, (double)p.pages) * p.ps * p.kvh * p.d * cache_bytes(p.kt) + 8.0 * p.tokens * (double)p.heads * p.d;
+    if (parts) {
+        p.split = blocks;
+        t.nblocks = blocks;
+        s->nargs = 7;
+    } else {
+        p.wpp = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
+        t.nblocks = (int)((passes * p.wpp + 7) / 8);
+        s->nargs = 6;
+    }
+    return true;
+}
+
+static bool build_beam(const std::string& op, const Attrs& a, KernelSpec* s) {
+    KTask& t = s->task;
+    BeamP& p = t.p.beam;
+    if (!need_between(a, "requests", 1, 1 << 20, &p.requests) || !need_between(a, "beams", 1, kBeamMax, &p.beams) ||
+        !need_between(a, "vocab", 1, 0x7fffffff / kBeamMax, &p.vocab))
+        return false;
+    const long long rows = (long long)p.requests * p.beams;
+    p.has_start = a.has("tokens");
+    if (rows > (1 << 20) || !maybe_between(a, "tokens", 1, 1 << 20, (int)rows, &p.tokens)) return false;
+    p.parts = beam_parts(p.vocab);
+    if (rows * p.parts > (1 << 30)) return false;
+    const double held = (double)rows * p.parts * beam_part_floats(p.beams);
+    if (op == "reef_beam_scan") {
+        t.family = F_BEAM_SCAN;
+        t.nblocks = (int)(rows * p.parts);
+        s->dyn_smem = (uint32_t)sizeof(BeamRoom<float>);
+        s->nargs = p.has_start ? 4 : 3;
+        s->flops = 4.0 * rows * p.vocab;
+        s->bytes = 4.0 * ((double)rows * p.vocab + held);
+        return true;
+    }
+    if (!need_between(a, "eos", 0, p.vocab - 1, &p.eos)) return false;
+    t.family = F_BEAM_PICK;
+    t.nblocks = p.requests;
+    s->dyn_smem = (uint32_t)beam_pick_smem();
+    s->nargs = p.has_start ? 8 : 7;
+    s->bytes = 4.0 * (held + 7.0 * rows);
+    return true;
 }
 
 // Build the device task + launch plan for a name.  Returns REEF_SUCC / REEF_NOT_FOUND.
@@ -316,6 +456,15 @@ static int build_spec(const std::string& name, KernelSpec* s) {
         plan_conv_simt(s);
         return REEF_SUCC;
     }
+    if (op == "reef_page_tables" || op == "reef_paged_append" || op == "reef_paged_attention" || op == "reef_paged_attention_parts" ||
+        op == "reef_paged_attention_join") {
+        if (!build_paged(op, a, s)) goto bad;
+        return REEF_SUCC;
+    }
+    if (op == "reef_beam_scan" || op == "reef_beam_pick") {
+        if (!build_beam(op, a, s)) goto bad;
+        return REEF_SUCC;
+    }
     // reef_conv2d_add_preact: conv + residual written to `out`, and relu(out + bias2) written to `out2` by the
     // same epilogue: the reference's fused_nn_conv2d_add followed by the next unit's fused_add_nn_relu
     // (resource/resnet152/resnet152.cu:340-363 and :2-12) in one launch.  args: in, weight, out, residual, bias2, out2.
@@ -499,6 +648,58 @@ static void fill_arg_bytes(KernelSpec* s) {
             if (p.i_out2 >= 0) b[p.i_out2] = f4((double)(p.ptot - 1) * p.pcs + p.poff + p.co);
             break;
         }
+        case F_PAGE_TABLES: {
+            const PagedP& p = t.p.paged;
+            const double R = p.rows, f = p.has_fork;
+            const double n[10] = {R * p.mp, R, R, R, R * p.mp, R, R + 1, 4.0 * p.tokens, R, 4.0 * R};
+            for (int i = 0; i < s->nargs; i++) b[i] = f4(n[i < 3 || f ? i : i + 1]);
+            break;
+        }
+        case F_PAGED_APPEND:
+        case F_PAGED_ATTENTION: {
+            const PagedP& p = t.p.paged;
+            const size_t cache = (size_t)p.pages * p.kvh * p.ps * p.d * (size_t)cache_bytes(p.kt);
+            int i = 0;
+            if (t.family == F_PAGED_APPEND) {
+                const double row = (double)p.kvh * p.d;
+                b[i++] = f4((p.tokens - 1.0) * p.qs + p.qo + row);
+                b[i++] = f4((p.tokens - 1.0) * p.vs + p.vo + row);
+                b[i++] = f4(4.0 * p.tokens);
+                if (p.has_fork) b[i++] = f4(4.0 * p.rows);
+                b[i++] = cache; b[i++] = cache;
+            } else {
+                const double row = (double)p.heads * p.d;
+                b[i++] = f4((p.tokens - 1.0) * p.qs + p.qo + row);
+                b[i++] = cache; b[i++] = cache;
+                b[i++] = f4((double)p.rows * p.mp);
+                b[i++] = f4(4.0 * p.tokens);
+                b[i++] = f4(p.tokens * row);
+                if (p.wpp == 0) b[i++] = paged_parts_bytes(p, t.nblocks);
+            }
+            break;
+        }
+        case F_PAGED_JOIN:
+            b[0] = paged_parts_bytes(t.p.paged, t.p.paged.split);
+            b[1] = f4((double)t.p.paged.tokens * t.p.paged.heads * t.p.paged.d);
+            break;
+        case F_BEAM_SCAN:
+        case F_BEAM_PICK: {
+            const BeamP& p = t.p.beam;
+            const double rows = (double)p.requests * p.beams, held = rows * p.parts * beam_part_floats(p.beams);
+            int i = 0;
+            if (t.family == F_BEAM_SCAN) {
+                b[i++] = f4((double)p.tokens * p.vocab);
+                b[i++] = f4(rows);
+                if (p.has_start) b[i++] = f4(rows + 1);
+                b[i++] = f4(held);
+            } else {
+                b[i++] = f4(held);
+                b[i++] = f4(rows); b[i++] = f4(rows);
+                if (p.has_start) b[i++] = f4(rows + 1);
+                while (i < s->nargs) b[i++] = f4(rows);
+            }
+            break;
+        }
         default:
             break;
     }
@@ -506,7 +707,7 @@ static void fill_arg_bytes(KernelSpec* s) {
 
 ArgUse arg_use(const KernelSpec& s, int arg) {
     const KTask& t = s.task;
-    int out = 0, out2 = -1;
+    int out = 0, out2 = -1, first_of = 1 << 20;   // first_of: this argument and all behind it are written
     ArgUse u = {0, 0, 0, 0};
     auto slice = [&](int c0, int c, int stride) {
         if (c < stride) { u.c0 = c0; u.c1 = c0 + c; u.stride = stride; }
@@ -544,10 +745,28 @@ ArgUse arg_use(const KernelSpec& s, int arg) {
             if (arg == 2) slice(t.p.conv.ooff, t.p.conv.co, t.p.conv.ocs);
             if (arg == out2) slice(t.p.conv.poff, t.p.conv.co, t.p.conv.pcs);
             break;
+        case F_PAGE_TABLES:
+            out = first_of = 3 + t.p.paged.has_fork;
+            break;
+        case F_PAGED_APPEND:
+            out = first_of = 3 + t.p.paged.has_fork;
+            break;
+        case F_PAGED_ATTENTION:
+            out = first_of = 5;
+            break;
+        case F_PAGED_JOIN:
+            out = 1;
+            break;
+        case F_BEAM_SCAN:
+            out = s.nargs - 1;
+            break;
+        case F_BEAM_PICK:
+            out = first_of = s.nargs - 4;
+            break;
         default:
             break;   // the other families write their first argument
     }
-    u.writes = arg == out || arg == out2;
+    u.writes = arg == out || arg == out2 || arg >= first_of;
     return u;
 }
 
@@ -590,6 +809,11 @@ __device__ __forceinline__ bool run_body(const KTask& t, int vb, unsigned char* 
     if (F == F_LAYERNORM) return body_layernorm(t, vb, smem, flag);
     if (F == F_ATTENTION) return attention_rows<false>(t, vb, smem, flag);
     if (F == F_ATTENTION_STAGED) return attention_rows<true>(t, vb, smem, flag);
+    if (F == F_PAGE_TABLES) return body_page_tables(t, vb, smem, flag);
+    if (F == F_PAGED_APPEND) return body_paged_append(t, vb, smem, flag);
+    if (F == F_PAGED_JOIN) return body_paged_join(t, vb, smem, flag);
+    if (F == F_BEAM_SCAN) return body_beam_scan(t, vb, smem, flag);
+    if (F == F_BEAM_PICK) return body_beam_pick(t, vb, smem, flag);
     return true;
 }
 
@@ -613,6 +837,11 @@ __device__ __noinline__ bool run_any(const KTask& t, int vb, unsigned char* smem
         case F_LAYERNORM: return run_body<F_LAYERNORM>(t, vb, smem, flag, EnterAlways());
         case F_ATTENTION:           // (the staged form for either: the dispatcher has 128 registers; same results bit for bit)
         case F_ATTENTION_STAGED: return run_body<F_ATTENTION_STAGED>(t, vb, smem, flag, EnterAlways());
+        case F_PAGE_TABLES: return run_body<F_PAGE_TABLES>(t, vb, smem, flag, EnterAlways());
+        case F_PAGED_APPEND: return run_body<F_PAGED_APPEND>(t, vb, smem, flag, EnterAlways());
+        case F_PAGED_JOIN: return run_body<F_PAGED_JOIN>(t, vb, smem, flag, EnterAlways());
+        case F_BEAM_SCAN: return run_body<F_BEAM_SCAN>(t, vb, smem, flag, EnterAlways());
+        case F_BEAM_PICK: return run_body<F_BEAM_PICK>(t, vb, smem, flag, EnterAlways());
         default: return true;
     }
 }
@@ -805,7 +1034,7 @@ void add_launches(unsigned long long n) { g_launches.fetch_add(n, std::memory_or
 #define FOR_EACH_FAMILY(X)                                                                      \
     X(F_MOCK_ADD) X(F_MOCK_MUL) X(F_FUSED_ADD_NCHW) X(F_BIAS_RELU) X(F_CONV_SIMT) X(F_MAX_POOL) \
     X(F_AVG_POOL) X(F_GLOBAL_AVG_POOL) X(F_COPY) X(F_DENSE) X(F_SOFTMAX) X(F_EMBEDDING) X(F_LAYERNORM) X(F_ATTENTION) X(F_ATTENTION_STAGED) \
-    X(F_NCHW_TO_NHWC4) X(F_IM2COL_NCHW)
+    X(F_NCHW_TO_NHWC4) X(F_IM2COL_NCHW) X(F_PAGE_TABLES) X(F_PAGED_APPEND) X(F_PAGED_JOIN) X(F_BEAM_SCAN) X(F_BEAM_PICK)
 
 static const void* plain_fn(int family) {
     switch (family) {
@@ -845,8 +1074,11 @@ static void prepare_carveout() {
     cudaFuncSetAttribute(be_fn(F_CONV_SIMT), cudaFuncAttributeMaxDynamicSharedMemorySize, kConvSimtSmem);
     cudaFuncSetAttribute(plain_fn(F_DENSE), cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
     cudaFuncSetAttribute(be_fn(F_DENSE), cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
+    cudaFuncSetAttribute(plain_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
+    cudaFuncSetAttribute(be_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
+    paged_prepare_device();
     cudaFuncSetAttribute((const void*)k_dispatch, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         std::max(att_smem(true), std::max(kDenseSmem, kConvSimtSmem)));
+                         std::max(std::max(att_smem(true), kPagedSmemMax), std::max(kDenseSmem, kConvSimtSmem)));
     int* w = nullptr;
     tc_error_word(&w);   // the device error word exists before any launch can be part of a stream capture
     cudaGetLastError();
@@ -940,12 +1172,19 @@ int make_chain(const KernelSpec* const* specs, void*** args, int n, int clusters
 
 int prepare_kernel(const KernelSpec& s, void** args) {
     prepare_carveout();
-    if (is_tc_family(s.task.family)) return bind_tc(s, args);
+    if (s.task.family == F_PAGED_ATTENTION) return paged_prepare_device();
+    if (is_own_family(s.task.family)) return bind_tc(s, args);
     return REEF_SUCC;
 }
 
 static int launch_tc(const KernelSpec& s, cudaStream_t st, void** args, const int* flag, int* slot, int tile_begin = 0,
                      int tile_count = -1) {
+    if (s.task.family == F_PAGED_ATTENTION) {
+        KTask t;
+        fill_args(s, args, &t);
+        count_launch();
+        return paged_launch(t, s.dyn_smem, st, flag, slot, tile_begin, tile_count);
+    }
     int rc = bind_tc(s, args);
     if (rc != REEF_SUCC) return rc;
     TcCache& c = *s.tc_cache;
@@ -959,7 +1198,7 @@ int launch_plain(const KernelSpec& s, const uint32_t dims[6], uint32_t smem, cud
         set_error("launch_params / shared_memory do not match the kernel plan of " + s.name);
         return REEF_OUT_OF_RANGE;
     }
-    if (is_tc_family(s.task.family)) return launch_tc(s, st, args, nullptr, nullptr);
+    if (is_own_family(s.task.family)) return launch_tc(s, st, args, nullptr, nullptr);
     KTask t;
     fill_args(s, args, &t);
     void* kargs[] = {&t};
@@ -975,7 +1214,7 @@ int launch_be(const KernelSpec& s, const uint32_t dims[6], uint32_t smem, cudaSt
         set_error("launch_params / shared_memory do not match the kernel plan of " + s.name);
         return REEF_OUT_OF_RANGE;
     }
-    if (is_tc_family(s.task.family)) return launch_tc(s, st, args, flag, slot);
+    if (is_own_family(s.task.family)) return launch_tc(s, st, args, flag, slot);
     KTask t;
     fill_args(s, args, &t);
     void* kargs[] = {&t, (void*)&flag, (void*)&slot};
@@ -1000,8 +1239,8 @@ int launch_dispatch(const KernelSpec* rt, void** rt_args, const KernelSpec* be, 
                     int be_num, int sm_partition, int occupancy, int num_sms, int* be_slot, int* ctrl, int* be_ctrl,
                     cudaStream_t st, cudaStream_t be_st) {
     if (be == nullptr) be_num = 0;
-    const bool rt_tc = rt != nullptr && is_tc_family(rt->task.family);
-    const bool be_tc = be_num > 0 && is_tc_family(be->task.family);
+    const bool rt_tc = rt != nullptr && is_own_family(rt->task.family);
+    const bool be_tc = be_num > 0 && is_own_family(be->task.family);
     if (occupancy < 1) occupancy = 1;
     if (be_num > 0 && (be_off < 0 || be_off + be_num > be->task.nblocks)) {
         set_error("best-effort block range outside the kernel");
@@ -1100,7 +1339,7 @@ int launch_dispatch_static(const KernelSpec* rt, void** rt_args, const KernelSpe
     }
     if (rt == nullptr && be == nullptr) return REEF_FAIL;
     if (be == nullptr) be_num = 0;
-    if ((rt != nullptr && is_tc_family(rt->task.family)) || (be_num > 0 && is_tc_family(be->task.family))) {
+    if ((rt != nullptr && is_own_family(rt->task.family)) || (be_num > 0 && is_own_family(be->task.family))) {
         set_error("reef_dispatch_static hosts logical-block kernels only (a tensor-core cluster kernel was given)");
         return REEF_FAIL;
     }
@@ -1159,6 +1398,9 @@ int kernel_attrs(const KernelSpec& s, reef_kernel_attrs_t* out) {
         if (rc != REEF_SUCC) return rc;
     } else if (s.task.family == F_ATTENTION_TC) {
         rc = att_func_attrs(&fa, &occ);
+        if (rc != REEF_SUCC) return rc;
+    } else if (s.task.family == F_PAGED_ATTENTION) {
+        rc = paged_func_attrs(s.task.p.paged, s.dyn_smem, &fa, &occ);
         if (rc != REEF_SUCC) return rc;
     } else {
         const void* fn = plain_fn(s.task.family);

@@ -71,6 +71,11 @@ int att_prepare_device();
 int att_launch(const AttParams& P, cudaStream_t st, const int* flag, int* slot, int head_begin = 0, int head_count = -1);
 int att_func_attrs(cudaFuncAttributes* fa, int* occ);
 
+// paged_attention.cu
+int paged_prepare_device();
+int paged_launch(const KTask& t, uint32_t smem, cudaStream_t st, const int* flag, int* slot, int first = 0, int count = -1);
+int paged_func_attrs(const PagedP& p, uint32_t smem, cudaFuncAttributes* fa, int* occ);
+
 // conv_tc_chain.cu: a run of tensor-core convolution layers as one persistent kernel
 struct TcChain;
 int chain_create(const std::vector<const TcParams*>& params, const std::vector<TcPlan>& plans, int clusters, TcChain** out);

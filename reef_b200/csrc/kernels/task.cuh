@@ -15,7 +15,7 @@
 namespace reef {
 
 constexpr int kThreads = 256;   // every family runs 256-thread blocks so the dispatcher can host any of them
-constexpr int kMaxArgs = 8;
+constexpr int kMaxArgs = 10;
 
 enum Family : int {
     F_MOCK_ADD = 0,
@@ -35,10 +35,16 @@ enum Family : int {
     F_ATTENTION_STAGED,
     F_NCHW_TO_NHWC4,
     F_IM2COL_NCHW,
+    F_PAGE_TABLES,
+    F_PAGED_APPEND,
+    F_PAGED_JOIN,
+    F_BEAM_SCAN,
+    F_BEAM_PICK,
     F_COUNT,
     // families with their own __global__ kernel (not hosted by the 256-thread logical-block wrappers)
     F_CONV_TC = 100,
-    F_ATTENTION_TC = 101
+    F_ATTENTION_TC = 101,
+    F_PAGED_ATTENTION = 102
 };
 
 // epilogue / option bits
@@ -76,6 +82,27 @@ struct SoftmaxP {
     int rows, n;
 };
 
+// operators of a decoding step over a paged key-value cache [page][key head][slot][dimension]
+enum : int { KT_FP32 = 0, KT_BF16 = 1, KT_FP16 = 2 };   // types of the cache
+struct PagedP {
+    int tokens, rows;        // tokens of the batch, rows of the page table
+    int heads, kvh, d;       // query heads, key heads, dimensions of a head
+    int ps, mp, pages, kt;   // tokens of a page, pages a row can have, pages of the cache, KT_*
+    int qs, qo, vs, vo;      // append: row stride and offset of the keys and of the values; attention: of the queries
+    int has_fork;            // page tables, append: rows continue from a parent row
+    int gb, subs;            // attention: query heads that share a pass over their keys, passes over a key head
+    int wpp;                 // attention without parts: warps that share a pass over a row; 0 = with parts
+    unsigned ps_mul;         // pos / ps = umulhi(2 pos, ps_mul) >> ps_shift for pos < 2^31
+    int ps_shift;
+    int split;               // page tables: blocks; append: blocks of tokens (the others copy forked pages)
+};
+struct BeamP {
+    int requests, beams, vocab, eos;
+    int tokens;              // rows of logits
+    int has_start;
+    int parts, part;         // parts of a row of logits, words of a part
+};
+
 struct KTask {
     int family;
     int nblocks;             // logical blocks of one launch
@@ -85,6 +112,8 @@ struct KTask {
         EltP elt;
         DenseP dense;
         SoftmaxP softmax;
+        PagedP paged;
+        BeamP beam;
         int raw[32];
     } p;
     void* a[kMaxArgs];       // device pointers, positional like the json "args"

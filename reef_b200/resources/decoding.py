@@ -1,0 +1,38 @@
+"""Kernel names of a decoding step over a paged key-value cache: which kernels an operator takes for a shape.
+
+Shared by the schedules (``decoder.py``) and by the operators on device tensors (``reef_b200/decode.py``).
+"""
+from __future__ import annotations
+
+from .graph import kname
+
+CACHE_TYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+
+
+def page_tables(rows: int, max_pages: int, page_size: int, pages: int, tokens: int, fork: bool) -> str:
+    """args: table, lens, new, [parent], table', lens', start, tok, status, [fork]"""
+    return kname("reef_page_tables", rows=rows, mp=max_pages, ps=page_size, pages=pages, tokens=tokens, **({"fork": 1} if fork else {}))
+
+
+def paged_append(tokens: int, kv_heads: int, dim: int, page_size: int, pages: int, cache: str, forks: int = 0, **strides) -> str:
+    """args: k, v, tok, [fork], k_cache, v_cache; ``strides``: ks, vs (floats from token to token), ko, vo (floats to the first)"""
+    return kname("reef_paged_append", tokens=tokens, kvh=kv_heads, d=dim, ps=page_size, pages=pages, kt=CACHE_TYPES[cache],
+                 **({"forks": forks} if forks else {}), **strides)
+
+
+def paged_attention(tokens: int, rows: int, heads: int, kv_heads: int, dim: int, page_size: int, max_pages: int, pages: int, cache: str,
+                    **strides) -> list:
+    """One name (args: q, k_cache, v_cache, table, tok, out), or two where the keys of a row are divided among blocks: the second
+    (args: parts, out) joins what the first (args: q, k_cache, v_cache, table, tok, out, parts) leaves in ``parts``.
+    ``strides``: qs (floats from token to token), qo (floats to the first)."""
+    shape = dict(tokens=tokens, rows=rows, heads=heads, kvh=kv_heads, d=dim, ps=page_size, mp=max_pages, pages=pages, kt=CACHE_TYPES[cache])
+    if max_pages * page_size <= 256:
+        return [kname("reef_paged_attention", **shape, **strides)]
+    return [kname("reef_paged_attention_parts", **shape, **strides), kname("reef_paged_attention_join", **shape)]
+
+
+def beam_select(requests: int, beams: int, vocab: int, eos: int, tokens: int | None = None) -> list:
+    """args: logits, live, [start], parts; then parts, score, live, [start], token, parent, score', live'"""
+    packed = {} if tokens is None else {"tokens": tokens}
+    return [kname("reef_beam_scan", requests=requests, beams=beams, vocab=vocab, **packed),
+            kname("reef_beam_pick", requests=requests, beams=beams, vocab=vocab, eos=eos, **packed)]
