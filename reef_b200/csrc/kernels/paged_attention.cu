@@ -14,8 +14,8 @@ namespace reef {
 extern __shared__ __align__(16) unsigned char reef_paged_smem[];
 
 // flag: best-effort flavour, else null; slot: completion counter, may be null; blocks [first, first + gridDim.x) of the kernel
-template <class E>
-__global__ void __launch_bounds__(kThreads, 2) k_paged_attention(const __grid_constant__ KTask t, int first, const int* flag, int* slot,
+template <class E, int BLOCKS>
+__global__ void __launch_bounds__(kThreads, BLOCKS) k_paged_attention(const __grid_constant__ KTask t, int first, const int* flag, int* slot,
                                                                  unsigned long long* stamps) {
     const int up = flag != nullptr && threadIdx.x == 0 ? ld_flag(flag) : 0;
     pdl_prologue();
@@ -36,17 +36,25 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_attention(const __grid_co
 }
 
 template <class C, int D>
-static const void* paged_fn_heads(int gb) {
-    switch (gb) {
-        case 1: return (const void*)k_paged_attention<PagedSimt<C, D, 1>>;
-        case 2: return (const void*)k_paged_attention<PagedSimt<C, D, 2>>;
-        case 4: return sizeof(C) == 4 ? (const void*)k_paged_attention<PagedSimt<float, D, 4>> : nullptr;
-        default: return nullptr;
+struct PagedFns {
+    static const void* of(int gb) {
+        return gb == 1 ? (const void*)k_paged_attention<PagedSimt<C, D, 1>, 2>
+             : gb == 2 ? (const void*)k_paged_attention<PagedSimt<C, D, 2>, 2>
+             : gb == 4 ? (const void*)k_paged_attention<PagedMma<C, D, 4>, D == 256 ? 1 : 2>
+             : gb == 8 ? (const void*)k_paged_attention<PagedMma<C, D, 8>, D == 256 ? 1 : 2> : nullptr;
     }
-}
+};
+template <int D>
+struct PagedFns<float, D> {
+    static const void* of(int gb) {
+        return gb == 1 ? (const void*)k_paged_attention<PagedSimt<float, D, 1>, 2>
+             : gb == 2 ? (const void*)k_paged_attention<PagedSimt<float, D, 2>, 2>
+             : gb == 4 ? (const void*)k_paged_attention<PagedSimt<float, D, 4>, 2> : nullptr;
+    }
+};
 template <class C>
 static const void* paged_fn_dim(int d, int gb) {
-    return d == 64 ? paged_fn_heads<C, 64>(gb) : d == 128 ? paged_fn_heads<C, 128>(gb) : d == 256 ? paged_fn_heads<C, 256>(gb) : nullptr;
+    return d == 64 ? PagedFns<C, 64>::of(gb) : d == 128 ? PagedFns<C, 128>::of(gb) : d == 256 ? PagedFns<C, 256>::of(gb) : nullptr;
 }
 static const void* paged_fn(const PagedP& p) {
     return p.kt == KT_FP32 ? paged_fn_dim<float>(p.d, p.gb) : p.kt == KT_BF16 ? paged_fn_dim<__nv_bfloat16>(p.d, p.gb) : paged_fn_dim<__half>(p.d, p.gb);
@@ -59,12 +67,12 @@ int paged_prepare_device() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16 || done[dev]) return REEF_SUCC;
     for (int kt = KT_FP32; kt <= KT_FP16; kt++)
         for (int d = 64; d <= 256; d *= 2)
-            for (int gb = 1; gb <= 4; gb *= 2) {
+            for (int gb = 1; gb <= 8; gb *= 2) {
                 PagedP p;
                 p.kt = kt; p.d = d; p.gb = gb;
                 const void* fn = paged_fn(p);
                 if (fn == nullptr) continue;
-                cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
+                cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_attention_smem(p));
                 if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
                 if (e != cudaSuccess) {
                     set_error(std::string("cudaFuncSetAttribute(paged attention): ") + cudaGetErrorString(e));

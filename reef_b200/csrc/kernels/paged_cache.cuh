@@ -25,7 +25,8 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // worked out by every block for itself (no block has to wait for another); each block then writes its own share of the rows.
 constexpr int kTablesMaxRows = 1024, kTablesMaxPages = 1 << 19;
 __host__ __device__ inline int tables_words(int pages) { return (pages + 31) / 32; }
-__host__ inline int tables_smem(int rows, int pages) { return 4 * (tables_words(pages) + 6 * rows + 2 + 32); }
+__host__ constexpr int tables_smem(int rows, int pages) { return 4 * ((pages + 31) / 32 + 6 * rows + 2 + 32); }
+constexpr int kTablesSmemMax = tables_smem(kTablesMaxRows, kTablesMaxPages);
 
 __device__ __forceinline__ int block_scan(int v, int* sums, int* total) {   // inclusive, over 256 threads in their order
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

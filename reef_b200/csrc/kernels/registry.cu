@@ -168,21 +168,22 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
     if (!need_between(a, "tokens", 1, 1 << 16, &p.tokens) || !need_between(a, "heads", 1, 1024, &p.heads) || !paged_heads(a, &p) || p.heads % p.kvh)
         return false;
     const int group = p.heads / p.kvh;
-    p.subs = ceil_div(group, paged_gb_max(p.kt, p.d));
-    p.gb = ceil_div(group, p.subs);
-    if (p.gb > 2) p.gb = 4;
+    p.gb = paged_heads_of_a_pass(p.kt, p.d, group);
+    p.subs = ceil_div(group, p.gb);
     if ((long long)p.tokens * p.kvh * p.subs > (1 << 30)) return false;
     const bool parts = op == "reef_paged_attention_parts", join = op == "reef_paged_attention_join";
     if (!need_between(a, "rows", 1, 1 << 16, &p.rows) || !paged_pages(a, &p) || !need_between(a, "mp", 1, (1 << 30) / p.ps, &p.mp)) return false;
+    if ((long long)p.pages * p.ps * p.kvh > 0x7fffffffLL) return false;   // a key's place is an int
     const long long passes = (long long)p.tokens * p.kvh * p.subs;
     const int units = ceil_div(p.mp * p.ps, paged_unit(p));
-    // With parts: two blocks to an SM, fewer where the longest rows would not give every warp its least work.
-    const int blocks = (int)std::min<long long>(2 * kSmsPlanned, (passes * units + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits));
+    if (passes * units > 0x70000000LL) return false;
+    // With parts: what the SMs hold at once, fewer where the longest rows would not give every warp its least work.
+    const int blocks = (int)std::min<long long>(paged_blocks_per_sm(p) * kSmsPlanned, (passes * units + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits));
     if (join) {
         p.split = blocks;
         t.family = F_PAGED_JOIN;
-        t.nblocks = blocks * p.gb;
-        s->dyn_smem = (uint32_t)paged_join_smem(p.d);
+        t.nblocks = paged_join_blocks(blocks, p.gb);
+        s->dyn_smem = (uint32_t)paged_join_smem(blocks);
         s->nargs = 2;
         s->bytes = (double)paged_parts_bytes(p, blocks);
         return true;
@@ -1074,11 +1075,11 @@ static void prepare_carveout() {
     cudaFuncSetAttribute(be_fn(F_CONV_SIMT), cudaFuncAttributeMaxDynamicSharedMemorySize, kConvSimtSmem);
     cudaFuncSetAttribute(plain_fn(F_DENSE), cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
     cudaFuncSetAttribute(be_fn(F_DENSE), cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
-    cudaFuncSetAttribute(plain_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
-    cudaFuncSetAttribute(be_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
+    cudaFuncSetAttribute(plain_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesSmemMax);
+    cudaFuncSetAttribute(be_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesSmemMax);
     paged_prepare_device();
     cudaFuncSetAttribute((const void*)k_dispatch, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         std::max(std::max(att_smem(true), kPagedSmemMax), std::max(kDenseSmem, kConvSimtSmem)));
+                         std::max(std::max(att_smem(true), kTablesSmemMax), std::max(kDenseSmem, kConvSimtSmem)));
     int* w = nullptr;
     tc_error_word(&w);   // the device error word exists before any launch can be part of a stream capture
     cudaGetLastError();
