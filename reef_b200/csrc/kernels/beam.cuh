@@ -10,10 +10,14 @@
 namespace reef {
 
 constexpr int kBeamMax = 16;
-constexpr int kBeamVecs = 4;                              // 128-bit loads of a thread and part
-constexpr int kBeamPart = kBeamVecs * 4 * kThreads;       // words of a part
+constexpr int kBeamVecs = 4;                              // 128-bit loads of a thread and turn
+constexpr int kBeamTurn = kBeamVecs * 4 * kThreads;       // words of a turn
 constexpr int kBeamRoom = 512;                            // candidates that are ranked side by side
-__host__ __device__ inline int beam_parts(int vocab) { return ((vocab + 3) / 4 + 1 + kBeamVecs * kThreads - 1) / (kBeamVecs * kThreads); }
+// Parts of a row of logits: four blocks to an SM over all rows, a turn to a part at least.
+__host__ inline int beam_parts(long long rows, int vocab) {
+    const long long turns = ((vocab + 3LL) / 4 + 1 + kBeamTurn / 4 - 1) / (kBeamTurn / 4), want = (4 * 148 + rows - 1) / rows;
+    return (int)(turns < want ? turns : want);
+}
 __host__ __device__ inline int beam_part_floats(int beams) { return 2 + 2 * beams; }
 
 template <class V>
@@ -22,6 +26,8 @@ struct BeamRoom {
     int index[kBeamRoom];
     V line[8];
     int who[8];
+    V best[2 * kBeamMax];
+    int best_index[2 * kBeamMax];
     int count;
 };
 constexpr int kBeamSmem = (int)sizeof(BeamRoom<double>);
@@ -109,14 +115,16 @@ __device__ __forceinline__ int beam_logits(const BeamP& p, const int* start, int
 }
 
 // ---- scan: a part of a row of logits -> its maximum, the sum of exponentials below it, its `beams` greatest ------------------
-// args: logits, live, [start], parts.  One pass: a part is held in registers, so the maximum, the sum and the selection look at it
-// without loading it again.  Bound by HBM (or L2, where the projection has just left the logits).
-__device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned char* smem, const int*) {
+// args: logits, live, [start], parts.  One pass: a thread carries a maximum and a sum of its own, the next turn's loads are under way while
+// a turn is looked at.  The first turn gives a line below which nothing counts any more; later turns add the few words above it
+// (words come in their order, so an equal one is too late), the line rises whenever the room is half full.  Bound by HBM (or L2, where the
+// projection has just left the logits).
+__device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned char* smem, const int* flag) {
     const BeamP& p = t.p.beam;
-    const int r = vb / p.parts, part = vb - r * p.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r = vb / p.parts, part = vb - r * p.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.beams;
     const int* live = (const int*)t.a[1];
     const int* start = p.has_start ? (const int*)t.a[2] : nullptr;
-    float* out = (float*)t.a[2 + p.has_start] + (size_t)vb * beam_part_floats(p.beams);
+    float* out = (float*)t.a[2 + p.has_start] + (size_t)vb * beam_part_floats(K);
     if (live[r] == 0) return true;
     const int row = beam_logits(p, start, r);
     if (row < 0) return true;
@@ -124,59 +132,143 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
     // loads begin at a 16-byte boundary: up to three words of the row before are masked
     const float* logits = (const float*)t.a[0] + (size_t)row * p.vocab;
     const int lead = (int)(((size_t)row * p.vocab) & 3);
-    float x[kBeamVecs][4];
+    const int begin = part * p.part * 4 - lead, end = min(p.vocab, begin + p.part * 4);
+    float x[kBeamVecs][4], next[kBeamVecs][4];
+    auto word = [&](int at, int i) { return at + (i * kThreads + tid) * 4; };        // first word of a load
+    auto load = [&](float (&y)[kBeamVecs][4], int at) {
 #pragma unroll
-    for (int i = 0; i < kBeamVecs; i++) {
-        const int w = ((part * kBeamVecs + i) * kThreads + tid) * 4 - lead;      // first word of this load
-        if (w >= 0 && w + 4 <= p.vocab) {
-            const float4 y = *reinterpret_cast<const float4*>(logits + w);
-            x[i][0] = y.x; x[i][1] = y.y; x[i][2] = y.z; x[i][3] = y.w;
-        } else {
+        for (int i = 0; i < kBeamVecs; i++) {
+            const int w = word(at, i);
+            if (w >= 0 && w + 4 <= end) {
+                const float4 v = *reinterpret_cast<const float4*>(logits + w);
+                y[i][0] = v.x; y[i][1] = v.y; y[i][2] = v.z; y[i][3] = v.w;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = w + e >= 0 && w + e < p.vocab ? logits[w + e] : -INFINITY;
+                for (int e = 0; e < 4; e++) y[i][e] = w + e >= 0 && w + e < end ? logits[w + e] : -INFINITY;
+            }
         }
-    }
-    float top = -INFINITY;
+    };
+    float top = -INFINITY, sum = 0.f, line = -INFINITY;
+    int here = begin, up = 0, have = 0;        // first word of this turn; candidates in the room
+    auto each = [&](auto f) {
 #pragma unroll
-    for (int i = 0; i < kBeamVecs; i++)
+        for (int i = 0; i < kBeamVecs; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, x[i][e]);
-    top = warp_max(top);
+            for (int e = 0; e < 4; e++) f(x[i][e], word(here, i) + e);
+    };
+    // the K greatest of the room's `count` go to its front, in their order
+    auto rank = [&](int count) {
+        float v[kBeamRoom / kThreads];
+        int w[kBeamRoom / kThreads], at[kBeamRoom / kThreads];
+#pragma unroll
+        for (int i = 0; i < kBeamRoom / kThreads; i++) {
+            const int c = tid + i * kThreads;
+            at[i] = K;
+            if (c < count) {
+                v[i] = s.value[c];
+                w[i] = s.index[c];
+                at[i] = 0;
+                for (int o = 0; o < count && at[i] < K; o++) at[i] += beam_before(s.value[o], s.index[o], v[i], w[i]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kBeamRoom / kThreads; i++)
+            if (at[i] < K) {
+                s.value[at[i]] = v[i];
+                s.index[at[i]] = w[i];
+            }
+        if (tid == 0) s.count = min(count, K);
+        __syncthreads();
+        if (count >= K) line = s.value[K - 1];
+        return min(count, K);
+    };
+    load(x, begin);
     __syncthreads();                           // a persistent caller's previous block is out of shared memory
-    if (lane == 0) s.line[warp] = top;
-    __syncthreads();
+    for (; here < end; here += kBeamTurn) {
+        if (flag != nullptr) {                 // best-effort flavour: a look at the preempt flag, asked for a turn ahead
+            if (__syncthreads_or(up)) return false;
+            up = tid == 0 ? ld_flag(flag) : 0;
+        }
+        if (here + kBeamTurn < end) load(next, here + kBeamTurn);
+        float high = top;
 #pragma unroll
-    for (int w = 0; w < 8; w++) top = fmaxf(top, s.line[w]);
-    float sum = 0.f;
+        for (int i = 0; i < kBeamVecs; i++) high = fmaxf(fmaxf(fmaxf(high, x[i][0]), fmaxf(x[i][1], x[i][2])), x[i][3]);
+        if (high > top) {
+            sum *= __expf(top - high);
+            top = high;
+        }
 #pragma unroll
-    for (int i = 0; i < kBeamVecs; i++)
+        for (int i = 0; i < kBeamVecs; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum += x[i][e] == -INFINITY ? 0.f : __expf(x[i][e] - top);
-    sum = warp_sum(sum);
-    __syncthreads();
-    if (lane == 0) s.value[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
+            for (int e = 0; e < 4; e++) sum += x[i][e] == -INFINITY ? 0.f : __expf(x[i][e] - top);
+        if (here == begin) {
+            have = block_top<float>(K, s, each, [&](int i, float v, int w) { s.best[i] = v; s.best_index[i] = w; });
+            __syncthreads();
+            if (tid < have) {
+                s.value[tid] = s.best[tid];
+                s.index[tid] = s.best_index[tid];
+            }
+            if (tid == 0) s.count = have;
+            if (have == K) line = s.best[K - 1];
+            __syncthreads();
+        } else {
+            each([&](float v, int w) {
+                if (v > line) {
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < kBeamRoom) {
+                        s.value[at] = v;
+                        s.index[at] = w;
+                    }
+                }
+            });
+            __syncthreads();
+            const int count = s.count;
+            __syncthreads();
+            if (count > kBeamRoom) {
+                // more than there is room for: what was there before, this turn by itself, and the two together
+                have = rank(have);
+                if (tid < have) {
+                    s.best[tid] = s.value[tid];
+                    s.best_index[tid] = s.index[tid];
+                }
+                __syncthreads();
+                const int found = block_top<float>(K, s, each, [&](int i, float v, int w) { s.best[have + i] = v; s.best_index[have + i] = w; });
+                __syncthreads();
+                have += found;
+                if (tid < have) {
+                    s.value[tid] = s.best[tid];
+                    s.index[tid] = s.best_index[tid];
+                }
+                __syncthreads();
+                have = rank(have);
+            } else {
+                have = count > kBeamRoom / 2 ? rank(count) : count;
+            }
+        }
 #pragma unroll
-    for (int w = 0; w < 8; w++) sum += s.value[w];
-    if (tid == 0) {
-        out[0] = top;
-        out[1] = sum;
+        for (int i = 0; i < kBeamVecs; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[i][e] = next[i][e];
     }
-    const int found = block_top<float>(p.beams, s,
-        [&](auto f) {
+    have = rank(have);
+    if (tid < K) {
+        out[2 + tid] = tid < have ? s.value[tid] : -INFINITY;
+        out[2 + K + tid] = __int_as_float(tid < have ? s.index[tid] : 0);
+    }
+    // all threads' sums
+    float high = warp_max(top);
+    if (lane == 0) s.line[warp] = high;
+    __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kBeamVecs; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) f(x[i][e], ((part * kBeamVecs + i) * kThreads + tid) * 4 - lead + e);
-        },
-        [&](int i, float v, int w) {
-            out[2 + i] = v;
-            out[2 + p.beams + i] = __int_as_float(w);
-        });
-    if (tid >= found && tid < p.beams) {
-        out[2 + tid] = -INFINITY;
-        out[2 + p.beams + tid] = __int_as_float(0);
+    for (int w = 0; w < 8; w++) high = fmaxf(high, s.line[w]);
+    sum = warp_sum(top == -INFINITY ? sum : sum * __expf(top - high));
+    if (lane == 0) s.best[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < 8; w++) sum += s.best[w];
+        out[0] = high;
+        out[1] = sum;
     }
     return true;
 }

@@ -21,31 +21,64 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // goes beyond; pages over the rows left, and those that need any are 1 from the one on that goes beyond.
 // The state goes from one set of buffers into another, so the kernel can be run again after a preemption.
 //
-// Nothing here moves many bytes: the time is that of the dependent steps (lengths, ids, prefix sums, rows).  The allocation is
-// worked out by every block for itself (no block has to wait for another); each block then writes its own share of the rows.
+// Nothing here moves many bytes: the time is that of the dependent steps (lengths, ids, prefix sums, ids again).  The allocation is
+// worked out by every block for itself, so that no block has to wait for another; the rows and tokens to write are divided.  Ids are read in
+// pieces of 128 of a row, eight pieces of a warp under way whatever the rows' lengths, and parents that several rows go on from once.
+// Used pages are marked in bytes, a window of the pages at a time, and packed to bits: an atomic OR into a word of bits took 1.5 cycles for
+// every id, 53 us for 62500 of them, a byte is a plain store.  A free page is found by its rank (a prefix sum over the threads' words, a walk
+// through one thread's), by whoever needs it.
 constexpr int kTablesMaxRows = 1024, kTablesMaxPages = 1 << 19;
-__host__ __device__ inline int tables_words(int pages) { return (pages + 31) / 32; }
-__host__ constexpr int tables_smem(int rows, int pages) { return 4 * ((pages + 31) / 32 + 6 * rows + 2 + 32); }
-constexpr int kTablesSmemMax = tables_smem(kTablesMaxRows, kTablesMaxPages);
+__host__ __device__ constexpr int tables_fixed(int rows, int pages) { return (4 * ((pages + 31) / 32 + 8 * rows + 3 + 24 + 260) + 15) / 16 * 16; }
+__host__ __device__ constexpr int tables_window(int rows, int pages) {      // what fits an SM beside the rest
+    const int all = (pages + 31) / 32 * 32, room = (225 * 1024 - tables_fixed(rows, pages)) / 512 * 512;
+    return all < room ? all : room;
+}
+__host__ constexpr int tables_smem(int rows, int pages) { return tables_fixed(rows, pages) + tables_window(rows, pages); }
+constexpr int kTablesSmemMax = 225 * 1024;
+// Rows and tokens are written by up to 32 blocks, 4096 ids or 256 tokens to a block.
+__host__ inline int tables_blocks(int rows, int max_pages, int tokens) {
+    const long long want = max(((long long)rows * max_pages + 4095) / 4096, (long long)(tokens + 255) / 256);
+    return (int)min(want, 32LL);
+}
 
-__device__ __forceinline__ int block_scan(int v, int* sums, int* total) {   // inclusive, over 256 threads in their order
+// inclusive sums over 256 threads in their order, of N values side by side; returns the exclusive ones in v, the totals in all
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&all)[N], int* sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
+    for (int n = 0; n < N; n++) {
+        x[n] = v[n];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, x[n], o);
+            if (lane >= o) x[n] += u;
+        }
     }
     __syncthreads();
-    if (lane == 31) sums[warp] = v;
-    __syncthreads();
-    int before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < 8; w++) {
-        if (w < warp) before += sums[w];
-        all += sums[w];
+    for (int n = 0; n < N; n++)
+        if (lane == 31) sums[8 * n + warp] = x[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        int before = 0;
+        all[n] = 0;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            if (w < warp) before += sums[8 * n + w];
+            all[n] += sums[8 * n + w];
+        }
+        v[n] = x[n] - v[n] + before;
     }
-    *total = all;
-    return v + before;
+}
+// the last i in [lo, hi) with a[i] <= x (a does not fall, a[lo] <= x)
+__device__ __forceinline__ int last_below(const int* a, int lo, int hi, int x) {
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
 }
 
 __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigned char* smem, const int*) {
@@ -61,151 +94,239 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
     int4* tok_out = (int4*)t.a[6 + f];
     int* status_out = (int*)t.a[7 + f];
     int4* fork_out = f ? (int4*)t.a[9] : nullptr;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = tables_words(N);
-    unsigned* used = (unsigned*)smem;              // a bit per page
-    int* sums = (int*)(used + words);              // 32 words of scratch
-    int* len = sums + 32;                          // per row: tokens held
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = (N + 31) / 32;
+    unsigned* open = (unsigned*)smem;              // a bit per page: used, later free
+    int* sums = (int*)(open + words);              // scratch of the prefix sums
+    int* holes = sums + 24;                        // free pages before every thread's words [256 + 1]
+    int* len = holes + 260;                        // per row: tokens held
     int* add = len + R;                            // tokens added
-    int* from = add + R;                           // row it goes on from
-    int* state = from + R;                         // status; then (accepted rows) 0
-    int* base = state + R;                         // rank of its first new page among the free ones [R + 1]
-    int* begin = base + R + 1;                     // first token [R + 1], also the lowest child of a row on the way
+    int* from = add + R;                           // row it goes on from, -1 for none
+    int* state = from + R;                         // status; -1 accepted with a copy of the last page
+    int* owner = state + R;                        // per parent: the lowest row that goes on from it
+    int* bad = owner + R;                          // per parent: an id out of range
+    int* base = bad + R;                           // rank of a row's first new page among the free ones [R + 1]; pieces of 32 ids before
+    int* begin = base + R + 1;                     // its first token [R + 1]
+    unsigned char* mark = smem + tables_fixed(R, N);      // a byte per page of a window
+    const int window = tables_window(R, N);
+    const bool wide = (M & 3) == 0 && ((uintptr_t)table & 15) == 0;         // rows begin at 16-byte boundaries
     __syncthreads();                               // a persistent caller's previous block is out of shared memory
-    for (int i = tid; i < words; i += kThreads) used[i] = 0;
     for (int r = tid; r < R; r += kThreads) {
         const int q = f ? parent[r] : r;
         const bool named = q >= -1 && q < R;
         const int l = named && q >= 0 ? lens[q] : 0, n = fresh[r];
         const bool good = named && l >= 0 && n >= 0 && (long long)l + n <= (long long)M * S;
-        len[r] = l; add[r] = n; from[r] = q;
+        len[r] = l; add[r] = n; from[r] = good ? q : -1;
         state[r] = good ? 0 : 2;
-        begin[r] = R;
+        owner[r] = f ? R : r;
+        bad[r] = 0;
     }
     __syncthreads();
-    // ids of the rows, a row to a warp: in range, and marked as used only where the whole row is good
-    for (int r = warp; r < R; r += 8) {
-        if (state[r]) continue;
-        const int l = len[r], kept = page_of(p, l + S - 1);
-        const int* ids = table + (size_t)max(from[r], 0) * M;
-        bool bad = false;
-        for (int j = lane; j < kept; j += 32) {
-            const int id = ids[j];
-            bad |= id < -1 || id >= N || (id < 0 && j == kept - 1 && l != kept * S);
-        }
-        bad = __any_sync(0xffffffffu, bad);
-        if (bad) {
-            if (lane == 0) state[r] = 2;
-            continue;
-        }
-        for (int j = lane; j < kept; j += 32) {
-            const int id = ids[j];
-            if (id >= 0) atomicOr(&used[id >> 5], 1u << (id & 31));
-        }
-        if (f && lane == 0 && from[r] >= 0) atomicMin(&begin[from[r]], r);
+    if (f) {
+        for (int r = tid; r < R; r += kThreads)
+            if (from[r] >= 0) atomicMin(&owner[from[r]], r);
+        __syncthreads();
     }
-    __syncthreads();
-    // sums over the rows: tokens, then pages of those whose tokens have room
+    // a thread's rows, at most four, in their order
     const int per = (R + kThreads - 1) / kThreads, r0 = tid * per, r1 = min(R, r0 + per);
-    int part = 0, all, have = 0;
-    const int wper = (words + kThreads - 1) / kThreads, w0 = tid * wper, w1 = min(words, w0 + wper);
-    for (int w = w0; w < w1; w++) have += __popc(used[w]);
-    const int holes = max(0, min(N, w1 * 32) - w0 * 32) - have;     // free pages among this thread's words
-    int frees;
-    const int hole0 = block_scan(w0 < w1 ? holes : 0, sums, &frees) - (w0 < w1 ? holes : 0);
+    auto kept = [&](int r) { return page_of(p, len[r] + S - 1); };
+    auto pieces = [&](int r) { return state[r] == 0 && from[r] >= 0 && owner[from[r]] == r ? (kept(r) + 127) >> 7 : 0; };
+    // bits of the pages that no row keeps; `part` of them among this thread's words
+    const int wper = (words + kThreads - 1) / kThreads, w0 = min(words, tid * wper), w1 = min(words, w0 + wper);
+    int part[3] = {0, 0, 0}, all[3];
+    for (int pass = 0; pass < 2; pass++) {         // (a second time without the rows whose ids are out of range, if there are any)
+        int count1[1] = {0}, all1[1];
+        for (int r = r0; r < r1; r++) count1[0] += pieces(r);
+        block_scan(count1, all1, sums);
+        for (int r = r0; r < r1; r++) {
+            base[r] = count1[0];
+            count1[0] += pieces(r);
+        }
+        if (tid == 0) base[R] = all1[0];
+        bool wrong = false;
+        for (int first = 0; first < N; first += window) {
+            for (int i = tid * 16; i < window; i += kThreads * 16) *reinterpret_cast<uint4*>(mark + i) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            for (int c0 = 0; c0 < all1[0]; c0 += kThreads) {
+                // every eighth piece to a warp, 32 of them at a time: a lane looks up the row of one
+                const int c = c0 + warp + 8 * lane;
+                int at = 0, left = 0, row = 0;
+                if (c < all1[0]) {
+                    row = last_below(base, 0, R, c);
+                    const int j = (c - base[row]) * 128;
+                    left = min(kept(row) - j, 129);
+                    at = from[row] * M + j;                                             // (rows * max_pages is at most 2^30)
+                    if (left <= 128 && len[row] != kept(row) * S) left |= 1 << 30;     // its last id names a page that is written
+                }
+                const int n = min(32, (all1[0] - c0 - warp + 7) >> 3);
+#pragma unroll 1
+                for (int i0 = 0; i0 < n; i0 += 8) {
+                    int4 id[8];
+                    int count[8];
+                    unsigned ill = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int* from4 = table + __shfl_sync(0xffffffffu, at, i0 + i) + 4 * lane;
+                        count[i] = __shfl_sync(0xffffffffu, left, i0 + i);       // (0 behind the last piece)
+                        const int m = min(count[i] & ~(1 << 30), 128) - 4 * lane;
+                        id[i] = make_int4(-1, -1, -1, -1);
+                        if (wide) {
+                            // (what lies behind the row's last id is looked away from below; the row of the table ends at 16 bytes)
+                            if (m > 0) id[i] = *reinterpret_cast<const int4*>(from4);
+                        } else {
+                            if (m > 0) id[i].x = from4[0];
+                            if (m > 1) id[i].y = from4[1];
+                            if (m > 2) id[i].z = from4[2];
+                            if (m > 3) id[i].w = from4[3];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int m = min(count[i] & ~(1 << 30), 128) - 4 * lane, written = count[i] & (1 << 30) ? m - 1 : -1;
+                        const int v[4] = {id[i].x, id[i].y, id[i].z, id[i].w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int x = e < m ? v[e] : -1;
+                            if (x < -1 || x >= N || (x < 0 && e == written)) ill |= 1u << i;
+                            if (x >= first && x - first < window) mark[x - first] = 1;
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, ill)) {
+                        wrong = true;
+#pragma unroll 1
+                        for (int i = 0; i < 8; i++) {
+                            const int r = __shfl_sync(0xffffffffu, row, i0 + i);
+                            if (__any_sync(0xffffffffu, ill >> i & 1) && lane == 0) bad[from[r]] = 1;
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            for (int w = tid; w < window / 32 && first / 32 + w < words; w += kThreads) {
+                const uint4* b = reinterpret_cast<const uint4*>(mark + w * 32);
+                unsigned x = 0;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint4 y = b[h];
+                    // the lowest bits of four bytes, by a product, as four bits
+                    x |= ((y.x * 0x10204080u) >> 28 | (y.y * 0x10204080u) >> 28 << 4 | (y.z * 0x10204080u) >> 28 << 8 | (y.w * 0x10204080u) >> 28 << 12) << 16 * h;
+                }
+                x = ~x;
+                if (first / 32 + w == words - 1 && (N & 31)) x &= (1u << (N & 31)) - 1;
+                open[first / 32 + w] = x;
+            }
+        }
+        if (!__syncthreads_or(wrong)) break;
+        for (int r = tid; r < R; r += kThreads)
+            if (from[r] >= 0 && bad[from[r]]) state[r] = 2;
+        __syncthreads();
+    }
+    for (int w = w0; w < w1; w++) part[0] += __popc(open[w]);
+    // sums over the rows: tokens, then pages of those whose tokens have room
     // (a length is at most 2^30, a sum over the rows goes beyond 32 bits: it stops counting where it is beyond any room)
     auto clipped = [](int a, int b) { return (int)min((long long)a + b, 0x1fffffLL); };
-    for (int r = r0; r < r1; r++) part = clipped(part, state[r] == 0 ? add[r] : 0);
-    int upto = block_scan(part, sums, &all) - part;
-    for (int r = r0; r < r1; r++) {
-        if (state[r]) continue;
-        upto = clipped(upto, add[r]);
-        if (upto > p.tokens) state[r] = 3;
+    auto forked = [&](int r) { return f && state[r] == 0 && from[r] >= 0 && len[r] != page_of(p, len[r]) * S && owner[from[r]] != r; };
+    auto needs = [&](int r) { return state[r] ? 0 : page_of(p, len[r] + add[r] + S - 1) - kept(r) + (forked(r) ? 1 : 0); };
+    auto count_rows = [&]() {
+        part[1] = part[2] = 0;
+        for (int r = r0; r < r1; r++) {
+            part[1] = clipped(part[1], state[r] == 0 ? add[r] : 0);
+            part[2] = clipped(part[2], needs(r));
+        }
+    };
+    count_rows();
+    int mine = part[0];
+    block_scan(part, all, sums);
+    holes[tid] = part[0];
+    const int frees = all[0];
+    if (all[1] > p.tokens) {
+        int upto = part[1];
+        for (int r = r0; r < r1; r++) {
+            if (state[r]) continue;
+            upto = clipped(upto, add[r]);
+            if (upto > p.tokens) state[r] = 3;
+        }
+        count_rows();
+        part[0] = mine;
+        block_scan(part, all, sums);
     }
-    auto forked = [&](int r) { return f && state[r] == 0 && from[r] >= 0 && len[r] != page_of(p, len[r]) * S && begin[from[r]] != r; };
-    auto needs = [&](int r) { return state[r] ? 0 : page_of(p, len[r] + add[r] + S - 1) - page_of(p, len[r] + S - 1) + (forked(r) ? 1 : 0); };
-    part = 0;
-    for (int r = r0; r < r1; r++) part = clipped(part, needs(r));
-    upto = block_scan(part, sums, &all) - part;
-    const int want = min(all, frees);
+    int upto = part[2];
     for (int r = r0; r < r1; r++) {
         const int n = needs(r);
         base[r] = upto;
         upto = clipped(upto, n);
         if (n > 0 && upto > frees) state[r] = 1;
     }
-    if (tid == 0) base[R] = all;
-    part = 0;
-    for (int r = r0; r < r1; r++) part += state[r] ? 0 : add[r];
-    upto = block_scan(part, sums, &all) - part;
-    // this block's rows; the lowest children are read for the last time
-    const int rows_per = (R + p.split - 1) / p.split, mine0 = min(R, vb * rows_per), mine1 = min(R, mine0 + rows_per);
-    unsigned fork_bits = 0;                         // of this thread's rows (at most four)
-    for (int r = r0; r < r1; r++) fork_bits |= forked(r) ? 1u << (r - r0) : 0;
-    __syncthreads();
+    if (all[2] > frees) {
+        part[0] = mine;
+        count_rows();
+        block_scan(part, all, sums);
+    }
+    upto = part[1];
     for (int r = r0; r < r1; r++) {
+        const bool copy = forked(r);
         begin[r] = upto;
         upto += state[r] ? 0 : add[r];
         if (state[r]) len[r] = add[r] = 0, from[r] = -1;
-        if (fork_bits >> (r - r0) & 1) state[r] = -1;   // accepted, with a copy
+        if (copy) state[r] = -1;
     }
-    if (tid == kThreads - 1) begin[R] = all;
+    if (tid == 0) begin[R] = all[1];
     __syncthreads();
-    // kept pages and the empty rest, a row to a warp
+    // the free page of a rank
+    auto free_page = [&](int rank) {
+        const int th = last_below(holes, 0, kThreads, rank);
+        int w = th * wper, left = rank - holes[th], n = __popc(open[w]);
+        while (left >= n) {
+            left -= n;
+            n = __popc(open[++w]);
+        }
+        unsigned x = open[w];
+        for (; left > 0; left--) x &= x - 1;
+        return w * 32 + __ffs(x) - 1;
+    };
+    // a row's j-th page: kept, or new
+    auto page_at = [&](int r, int j) {
+        const int copied = kept(r) - (state[r] < 0 ? 1 : 0);
+        return j < copied ? table[(size_t)from[r] * M + j] : free_page(base[r] + j - copied);
+    };
+    const int rows_per = (R + p.split - 1) / p.split, mine0 = min(R, vb * rows_per), mine1 = min(R, mine0 + rows_per);
     for (int r = mine0 + warp; r < mine1; r += 8) {
-        const int q = from[r], kept = page_of(p, len[r] + S - 1), total = page_of(p, len[r] + add[r] + S - 1);
-        const int copied = state[r] < 0 ? kept - 1 : kept;
-        const int* ids = table + (size_t)max(q, 0) * M;
-        for (int j = lane; j < M; j += 32)
-            if (j < copied || j >= total) table_out[(size_t)r * M + j] = j < copied ? ids[j] : -1;
-    }
-    // free pages by rank: every thread's words hold the ranks from hole0 on
-    if (hole0 < want) {
-        int rank = hole0, r = 0;
-        {   // the last row that begins at or before this rank
-            int hi = R;
-            while (hi - r > 1) {
-                const int mid = (r + hi) >> 1;
-                if (base[mid] <= rank) r = mid; else hi = mid;
+        const int total = page_of(p, len[r] + add[r] + S - 1), copied = kept(r) - (state[r] < 0 ? 1 : 0);
+        const int* ids = table + (size_t)max(from[r], 0) * M;
+        int* to = table_out + (size_t)r * M;
+#pragma unroll 1
+        for (int j0 = lane; j0 < M; j0 += 256) {
+            int id[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = j0 + 32 * i;
+                id[i] = j < copied ? ids[j] : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = j0 + 32 * i;
+                if (j < M && (j < copied || j >= total)) to[j] = id[i];
             }
         }
-        for (int w = w0; w < w1 && rank < want; w++) {
-            unsigned open = ~used[w];
-            if (w == words - 1 && (N & 31)) open &= (1u << (N & 31)) - 1;
-            while (open && rank < want) {
-                const int id = w * 32 + __ffs(open) - 1;
-                open &= open - 1;
-                while (r + 1 < R && base[r + 1] <= rank) r++;
-                if (r >= mine0 && r < mine1 && state[r] <= 0) {
-                    const int j = page_of(p, len[r] + S - 1) + (state[r] < 0 ? -1 : 0) + rank - base[r];
-                    if (j < M) table_out[(size_t)r * M + j] = id;
-                }
-                rank++;
-            }
-        }
+        for (int j = copied + lane; j < total; j += 32) to[j] = free_page(base[r] + j - copied);
     }
-    __syncthreads();
     for (int r = mine0 + tid; r < mine1; r += kThreads) {
         lens_out[r] = len[r] + add[r];
         start_out[r] = begin[r];
         status_out[r] = max(state[r], 0);
         if (f) {
-            const int kept = page_of(p, len[r] + S - 1);
-            int4 c = make_int4(-1, -1, 0, 0);
-            if (state[r] < 0) c = make_int4(table[(size_t)from[r] * M + kept - 1], table_out[(size_t)r * M + kept - 1], len[r] - (kept - 1) * S, 0);
-            fork_out[r] = c;
+            const int k = kept(r);
+            fork_out[r] = state[r] < 0 ? make_int4(table[(size_t)from[r] * M + k - 1], page_at(r, k - 1), len[r] - (k - 1) * S, 0) : make_int4(-1, -1, 0, 0);
         }
     }
     if (vb == 0 && tid == 0) start_out[R] = begin[R];
-    for (int i = begin[mine0] + tid; i < begin[mine1]; i += kThreads) {
-        int r = mine0, hi = mine1;
-        while (hi - r > 1) {
-            const int mid = (r + hi) >> 1;
-            if (begin[mid] <= i) r = mid; else hi = mid;
+    for (int i = vb * kThreads + tid; i < p.tokens; i += p.split * kThreads) {
+        int4 x = make_int4(-1, -1, 0, 0);
+        if (i < begin[R]) {
+            const int r = last_below(begin, 0, R, i), pos = len[r] + i - begin[r], j = page_of(p, pos);
+            x = make_int4(page_at(r, j) * S + pos - j * S, r, pos + 1, 0);
         }
-        const int pos = len[r] + i - begin[r], j = page_of(p, pos);
-        tok_out[i] = make_int4(table_out[(size_t)r * M + j] * S + pos - j * S, r, pos + 1, 0);
+        tok_out[i] = x;
     }
-    for (int i = begin[R] + vb * kThreads + tid; i < p.tokens; i += p.split * kThreads) tok_out[i] = make_int4(-1, -1, 0, 0);
     return true;
 }
 

@@ -137,8 +137,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
             p.pages > kTablesMaxPages || !need_between(a, "mp", 1, (1 << 30) / p.ps, &p.mp) || (long long)p.rows * p.mp > (1 << 30))
             return false;
         p.has_fork = a.get("fork", 0) != 0;
-        // Rows are written by up to 32 blocks, 4096 ids to a block; what comes before is done by each of them.
-        p.split = (int)std::min<long long>(std::min(32, p.rows), ((long long)p.rows * p.mp + 4095) / 4096);
+        p.split = tables_blocks(p.rows, p.mp, p.tokens);
         t.family = F_PAGE_TABLES;
         t.nblocks = p.split;
         s->dyn_smem = (uint32_t)tables_smem(p.rows, p.pages);
@@ -217,7 +216,8 @@ static bool build_beam(const std::string& op, const Attrs& a, KernelSpec* s) {
     const long long rows = (long long)p.requests * p.beams;
     p.has_start = a.has("tokens");
     if (rows > (1 << 20) || !maybe_between(a, "tokens", 1, 1 << 20, (int)rows, &p.tokens)) return false;
-    p.parts = beam_parts(p.vocab);
+    p.parts = beam_parts(rows, p.vocab);
+    p.part = (int)((((long long)p.vocab + 3) / 4 + 1 + p.parts - 1) / p.parts);      // 128-bit loads of a part
     if (rows * p.parts > (1 << 30)) return false;
     const double held = (double)rows * p.parts * beam_part_floats(p.beams);
     if (op == "reef_beam_scan") {
@@ -865,7 +865,7 @@ __device__ __forceinline__ void preempt_stamp_leave() {
 }
 
 // Two blocks per SM where the body's registers would otherwise leave room for one.
-constexpr int min_blocks(int family) { return family == F_CONV_SIMT || family == F_ATTENTION_STAGED ? 2 : 1; }
+constexpr int min_blocks(int family) { return family == F_CONV_SIMT || family == F_ATTENTION_STAGED ? 2 : family == F_BEAM_SCAN ? 3 : 1; }
 
 template <int F>
 __global__ void __launch_bounds__(kThreads, min_blocks(F)) k_plain(const __grid_constant__ KTask t) {

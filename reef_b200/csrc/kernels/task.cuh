@@ -100,7 +100,7 @@ struct BeamP {
     int requests, beams, vocab, eos;
     int tokens;              // rows of logits
     int has_start;
-    int parts, part;         // parts of a row of logits, words of a part
+    int parts, part;         // parts of a row of logits, 128-bit loads of a part
 };
 
 struct KTask {
