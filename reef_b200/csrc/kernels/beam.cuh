@@ -5,18 +5,21 @@
 // finite score.  What is missing comes
 // out as token -1, parent -1, score -infinity, live 0.
 #pragma once
-#include "simple.cuh"
+#include "paged_cache.cuh"
 
 namespace reef {
 
 constexpr int kBeamMax = 16;
-constexpr int kBeamVecs = 4;                              // 128-bit loads of a thread and turn
-constexpr int kBeamTurn = kBeamVecs * 4 * kThreads;       // words of a turn
-constexpr int kBeamRoom = 512;                            // candidates that are ranked side by side
-// Parts of a row of logits: four blocks to an SM over all rows, a turn to a part at least.
+constexpr int kBeamVecs = 4;                              // 128-bit loads of a lane and turn
+constexpr int kBeamTurn = kBeamVecs * 4 * 32;             // words of a warp's turn
+constexpr int kBeamRoom = 512;                            // candidates that a block ranks side by side
+// Parts of a row of logits, a part to a block: a turn of its eight warps at least, and over all rows not more blocks than four to an SM
+// or, from there on, whole rounds of as many.
 __host__ inline int beam_parts(long long rows, int vocab) {
-    const long long turns = ((vocab + 3LL) / 4 + 1 + kBeamTurn / 4 - 1) / (kBeamTurn / 4), want = (4 * 148 + rows - 1) / rows;
-    return (int)(turns < want ? turns : want);
+    const long long least = 8LL * kBeamTurn, most = (vocab + least - 1) / least, slots = 4 * 148;
+    if (rows * most <= slots) return (int)most;
+    if (rows <= slots) return (int)(slots / rows);
+    return 1;
 }
 __host__ __device__ inline int beam_part_floats(int beams) { return 2 + 2 * beams; }
 
@@ -26,8 +29,6 @@ struct BeamRoom {
     int index[kBeamRoom];
     V line[8];
     int who[8];
-    V best[2 * kBeamMax];
-    int best_index[2 * kBeamMax];
     int count;
 };
 constexpr int kBeamSmem = (int)sizeof(BeamRoom<double>);
@@ -115,10 +116,22 @@ __device__ __forceinline__ int beam_logits(const BeamP& p, const int* start, int
 }
 
 // ---- scan: a part of a row of logits -> its maximum, the sum of exponentials below it, its `beams` greatest ------------------
-// args: logits, live, [start], parts.  One pass: a thread carries a maximum and a sum of its own, the next turn's loads are under way while
-// a turn is looked at.  The first turn gives a line below which nothing counts any more; later turns add the few words above it
-// (words come in their order, so an equal one is too late), the line rises whenever the room is half full.  Bound by HBM (or L2, where the
-// projection has just left the logits).
+// args: logits, live, [start], parts.  One pass, a range of the part to a warp, no warp waiting for another until the end: a lane carries a
+// maximum and a sum of its own, the next turn's loads are under way while a turn is looked at.  The greatest words so far stand in their
+// order in the warp's first K lanes; a word that is greater than the last of them moves in by a shuffle.  What keeps that rare: the first
+// turn begins with the K-th greatest of the lanes' maxima as a line, and the greatest line of the block's warps holds for all of them.
+// Bound by HBM (or L2, where the projection has just left the logits) as long as few words move in.
+struct BeamScan {
+    float value[8][kBeamMax];
+    int index[8][kBeamMax];
+    float top[8], sum[8];
+    float line;                  // K words of the part are at or above it
+};
+__device__ __forceinline__ float2 exp_two(float x, float y, float top) {     // e^(x - top), e^(y - top)
+    float2 d = add2(make_float2(x, y), make_float2(-top, -top));
+    d = fma2(d, make_float2(kLog2e, kLog2e), make_float2(0.f, 0.f));
+    return make_float2(exp2_fast(d.x), exp2_fast(d.y));
+}
 __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned char* smem, const int* flag) {
     const BeamP& p = t.p.beam;
     const int r = vb / p.parts, part = vb - r * p.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.beams;
@@ -128,147 +141,159 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
     if (live[r] == 0) return true;
     const int row = beam_logits(p, start, r);
     if (row < 0) return true;
-    BeamRoom<float>& s = *reinterpret_cast<BeamRoom<float>*>(smem);
+    BeamScan& s = *reinterpret_cast<BeamScan*>(smem);
     // loads begin at a 16-byte boundary: up to three words of the row before are masked
     const float* logits = (const float*)t.a[0] + (size_t)row * p.vocab;
     const int lead = (int)(((size_t)row * p.vocab) & 3);
-    const int begin = part * p.part * 4 - lead, end = min(p.vocab, begin + p.part * 4);
-    float x[kBeamVecs][4], next[kBeamVecs][4];
-    auto word = [&](int at, int i) { return at + (i * kThreads + tid) * 4; };        // first word of a load
-    auto load = [&](float (&y)[kBeamVecs][4], int at) {
+    const int first = part * p.part, loads = min(p.part, (p.vocab + lead + 3) / 4 - first);         // 128-bit loads of this part
+    const int each_warp = loads > 0 ? ((loads + 7) / 8 + 31) / 32 * 32 : 0;
+    const int begin = (first + warp * each_warp) * 4 - lead, end = min(p.vocab, (first + min(loads, (warp + 1) * each_warp)) * 4 - lead);
+    float4 x[kBeamVecs], next[kBeamVecs];
+    auto load = [&](float4 (&y)[kBeamVecs], int at) {
 #pragma unroll
         for (int i = 0; i < kBeamVecs; i++) {
-            const int w = word(at, i);
+            const int w = at + (i * 32 + lane) * 4;
             if (w >= 0 && w + 4 <= end) {
-                const float4 v = *reinterpret_cast<const float4*>(logits + w);
-                y[i][0] = v.x; y[i][1] = v.y; y[i][2] = v.z; y[i][3] = v.w;
+                y[i] = *reinterpret_cast<const float4*>(logits + w);
             } else {
+                float z[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[i][e] = w + e >= 0 && w + e < end ? logits[w + e] : -INFINITY;
+                for (int e = 0; e < 4; e++) z[e] = w + e >= 0 && w + e < end ? logits[w + e] : -INFINITY;
+                y[i] = make_float4(z[0], z[1], z[2], z[3]);
             }
         }
     };
-    float top = -INFINITY, sum = 0.f, line = -INFINITY;
-    int here = begin, up = 0, have = 0;        // first word of this turn; candidates in the room
-    auto each = [&](auto f) {
-#pragma unroll
-        for (int i = 0; i < kBeamVecs; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) f(x[i][e], word(here, i) + e);
-    };
-    // the K greatest of the room's `count` go to its front, in their order
-    auto rank = [&](int count) {
-        float v[kBeamRoom / kThreads];
-        int w[kBeamRoom / kThreads], at[kBeamRoom / kThreads];
-#pragma unroll
-        for (int i = 0; i < kBeamRoom / kThreads; i++) {
-            const int c = tid + i * kThreads;
-            at[i] = K;
-            if (c < count) {
-                v[i] = s.value[c];
-                w[i] = s.index[c];
-                at[i] = 0;
-                for (int o = 0; o < count && at[i] < K; o++) at[i] += beam_before(s.value[o], s.index[o], v[i], w[i]);
-            }
+    int here = begin;                          // first word of this turn
+    float top = -INFINITY;
+    float2 sum = make_float2(0.f, 0.f);
+    // this lane's word among the K greatest; the last of them
+    float mine = -INFINITY, last = -INFINITY;
+    int mine_i = 0x7fffffff, last_i = 0x7fffffff;
+    auto move_in = [&](float v, int w) {       // (the same v and w in all lanes; it comes before the last)
+        const int at = __popc(__ballot_sync(0xffffffffu, lane < K && beam_before(mine, mine_i, v, w)));
+        const float pv = __shfl_up_sync(0xffffffffu, mine, 1);
+        const int pi = __shfl_up_sync(0xffffffffu, mine_i, 1);
+        if (lane >= at) {
+            mine = lane == at ? v : pv;
+            mine_i = lane == at ? w : pi;
         }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kBeamRoom / kThreads; i++)
-            if (at[i] < K) {
-                s.value[at[i]] = v[i];
-                s.index[at[i]] = w[i];
-            }
-        if (tid == 0) s.count = min(count, K);
-        __syncthreads();
-        if (count >= K) line = s.value[K - 1];
-        return min(count, K);
+        last = __shfl_sync(0xffffffffu, mine, K - 1);
+        last_i = __shfl_sync(0xffffffffu, mine_i, K - 1);
     };
+    // the greatest line of the block's warps: as an integer a float >= 0 keeps its order, a float < 0 has it turned round
+    auto raise = [&](float v) {
+        if (v >= 0.f) atomicMax((int*)&s.line, __float_as_int(v));
+        else atomicMin((unsigned*)&s.line, __float_as_uint(v));
+    };
+    bool stopped = false;
+    int up = 0, turns = 0;
     load(x, begin);
     __syncthreads();                           // a persistent caller's previous block is out of shared memory
+    if (tid == 0) s.line = -INFINITY;
+    __syncthreads();
+#pragma unroll 1
     for (; here < end; here += kBeamTurn) {
-        if (flag != nullptr) {                 // best-effort flavour: a look at the preempt flag, asked for a turn ahead
-            if (__syncthreads_or(up)) return false;
-            up = tid == 0 ? ld_flag(flag) : 0;
+        if (flag != nullptr && (++turns & 3) == 0) {       // best-effort flavour: a look at the preempt flag, asked for ahead
+            if (__any_sync(0xffffffffu, up)) {
+                stopped = true;
+                break;
+            }
+            up = ld_flag(flag);
         }
         if (here + kBeamTurn < end) load(next, here + kBeamTurn);
-        float high = top;
+        float h[kBeamVecs];
 #pragma unroll
-        for (int i = 0; i < kBeamVecs; i++) high = fmaxf(fmaxf(fmaxf(high, x[i][0]), fmaxf(x[i][1], x[i][2])), x[i][3]);
+        for (int i = 0; i < kBeamVecs; i++) h[i] = fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w));
+        const float high = fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3]));
         if (high > top) {
-            sum *= __expf(top - high);
+            const float by = exp2_fast((top - high) * kLog2e);
+            sum.x *= by;
+            sum.y *= by;
             top = high;
         }
+        if (top == -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < kBeamVecs; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += x[i][e] == -INFINITY ? 0.f : __expf(x[i][e] - top);
-        if (here == begin) {
-            have = block_top<float>(K, s, each, [&](int i, float v, int w) { s.best[i] = v; s.best_index[i] = w; });
-            __syncthreads();
-            if (tid < have) {
-                s.value[tid] = s.best[tid];
-                s.index[tid] = s.best_index[tid];
+            for (int i = 0; i < kBeamVecs; i++) {       // (a NaN is not lost)
+                const float v = x[i].x + x[i].y + x[i].z + x[i].w;
+                if (v != v) sum.x += v;
             }
-            if (tid == 0) s.count = have;
-            if (have == K) line = s.best[K - 1];
-            __syncthreads();
         } else {
-            each([&](float v, int w) {
-                if (v > line) {
-                    const int at = atomicAdd(&s.count, 1);
-                    if (at < kBeamRoom) {
-                        s.value[at] = v;
-                        s.index[at] = w;
-                    }
-                }
-            });
-            __syncthreads();
-            const int count = s.count;
-            __syncthreads();
-            if (count > kBeamRoom) {
-                // more than there is room for: what was there before, this turn by itself, and the two together
-                have = rank(have);
-                if (tid < have) {
-                    s.best[tid] = s.value[tid];
-                    s.best_index[tid] = s.index[tid];
-                }
-                __syncthreads();
-                const int found = block_top<float>(K, s, each, [&](int i, float v, int w) { s.best[have + i] = v; s.best_index[have + i] = w; });
-                __syncthreads();
-                have += found;
-                if (tid < have) {
-                    s.value[tid] = s.best[tid];
-                    s.index[tid] = s.best_index[tid];
-                }
-                __syncthreads();
-                have = rank(have);
-            } else {
-                have = count > kBeamRoom / 2 ? rank(count) : count;
+#pragma unroll
+            for (int i = 0; i < kBeamVecs; i++) {
+                const float2 a = exp_two(x[i].x, x[i].y, top), b = exp_two(x[i].z, x[i].w, top);
+                sum = add2(sum, add2(a, b));
             }
         }
+        float line = *(volatile float*)&s.line;        // nothing below it counts, in this warp or another
+        if (here == begin) {
+            int rank = 0;
 #pragma unroll
-        for (int i = 0; i < kBeamVecs; i++)
+            for (int j = 0; j < 32; j++) {
+                const float v = __shfl_sync(0xffffffffu, high, j);
+                rank += v > high || (v == high && j < lane);
+            }
+            line = fmaxf(line, __shfl_sync(0xffffffffu, high, __ffs(__ballot_sync(0xffffffffu, rank == K - 1)) - 1));
+        }
+        // (an equal word of this warp's later turns is too late; among one turn's, and another warp's, it need not be)
+        auto counts = [&](float v, int w) { return v >= line && v > -INFINITY && beam_before(v, w, last, last_i); };
+        if (__any_sync(0xffffffffu, high >= line && high > -INFINITY && high >= last)) {
+            const float before = last;
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = next[i][e];
+            for (int i = 0; i < kBeamVecs; i++) {
+                if (!__any_sync(0xffffffffu, h[i] >= line && h[i] >= last)) continue;
+                const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                const int w = here + (i * 32 + lane) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    unsigned m = __ballot_sync(0xffffffffu, counts(v[e], w + e));
+                    while (m) {
+                        const int src = __ffs(m) - 1;
+                        move_in(__shfl_sync(0xffffffffu, v[e], src), __shfl_sync(0xffffffffu, w + e, src));
+                        m &= m - 1;
+                        m &= __ballot_sync(0xffffffffu, counts(v[e], w + e));
+                    }
+                }
+            }
+            if (lane == 0 && last > before && last > line) raise(last);
+        }
+#pragma unroll
+        for (int i = 0; i < kBeamVecs; i++) x[i] = next[i];
     }
-    have = rank(have);
-    if (tid < K) {
-        out[2 + tid] = tid < have ? s.value[tid] : -INFINITY;
-        out[2 + K + tid] = __int_as_float(tid < have ? s.index[tid] : 0);
-    }
-    // all threads' sums
+    // the warps' sums and candidates meet
     float high = warp_max(top);
-    if (lane == 0) s.line[warp] = high;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) high = fmaxf(high, s.line[w]);
-    sum = warp_sum(top == -INFINITY ? sum : sum * __expf(top - high));
-    if (lane == 0) s.best[warp] = sum;
-    __syncthreads();
+    const float part_sum = sum.x + sum.y, total = warp_sum(top == -INFINITY ? part_sum : part_sum * exp2_fast((top - high) * kLog2e));
+    if (lane == 0) {
+        s.top[warp] = high;
+        s.sum[warp] = total;
+    }
+    if (lane < K) {
+        s.value[warp][lane] = mine;
+        s.index[warp][lane] = mine_i;
+    }
+    if (__syncthreads_or(stopped)) return false;
     if (tid == 0) {
-        for (int w = 1; w < 8; w++) sum += s.best[w];
+        float all = 0.f;
+        for (int w = 0; w < 8; w++) high = fmaxf(high, s.top[w]);
+        for (int w = 0; w < 8; w++) all += s.top[w] == -INFINITY ? s.sum[w] : s.sum[w] * exp2_fast((s.top[w] - high) * kLog2e);
         out[0] = high;
-        out[1] = sum;
+        out[1] = all;
+    }
+    if (tid < 8 * K) {
+        // a candidate's place: how many come before it; those that are none stand behind them, the lowest first
+        const int w = tid / K, c = tid - w * K, index = s.index[w][c];
+        const float v = s.value[w][c];
+        int at = 0;
+#pragma unroll
+        for (int o = 0; o < 8; o++)
+            for (int k = 0; k < K; k++) {
+                const float u = s.value[o][k];
+                const int i = s.index[o][k];
+                at += beam_before(u, i, v, index) || (u == v && i == index && o * K + k < tid);
+            }
+        if (at < K) {
+            out[2 + at] = v;
+            out[2 + K + at] = __int_as_float(index);
+        }
     }
     return true;
 }

@@ -223,7 +223,7 @@ static bool build_beam(const std::string& op, const Attrs& a, KernelSpec* s) {
     if (op == "reef_beam_scan") {
         t.family = F_BEAM_SCAN;
         t.nblocks = (int)(rows * p.parts);
-        s->dyn_smem = (uint32_t)sizeof(BeamRoom<float>);
+        s->dyn_smem = (uint32_t)sizeof(BeamScan);
         s->nargs = p.has_start ? 4 : 3;
         s->flops = 4.0 * rows * p.vocab;
         s->bytes = 4.0 * ((double)rows * p.vocab + held);
@@ -865,7 +865,7 @@ __device__ __forceinline__ void preempt_stamp_leave() {
 }
 
 // Two blocks per SM where the body's registers would otherwise leave room for one.
-constexpr int min_blocks(int family) { return family == F_CONV_SIMT || family == F_ATTENTION_STAGED ? 2 : family == F_BEAM_SCAN ? 3 : 1; }
+constexpr int min_blocks(int family) { return family == F_CONV_SIMT || family == F_ATTENTION_STAGED ? 2 : family == F_BEAM_SCAN ? 4 : 1; }
 
 template <int F>
 __global__ void __launch_bounds__(kThreads, min_blocks(F)) k_plain(const __grid_constant__ KTask t) {
