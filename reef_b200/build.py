@@ -1,8 +1,9 @@
-"""In-tree build of the two shared libraries.
+"""In-tree build of the shared libraries.
 
 ``libreef_cuda.so``  C-ABI device layer + every CUDA kernel, nvcc for sm_100a only.
 ``libreef_host.so``  C++ host side (loader, executors, scheduler) + its C entry points, linked
                      against libreef_cuda.so through the C-ABI header only.
+``_decode.so``       the decoding operators' calls on torch tensors (``decode.py``), over the same header.
 
 A content hash of sources and flags is stored beside each library so that an up-to-date
 library (for instance one that travelled to a GPU machine with the source tree) is not rebuilt.
@@ -90,8 +91,29 @@ def build_host(verbose: bool = False) -> str:
     return out
 
 
+def build_torch(verbose: bool = False) -> str:
+    """The calls of ``decode.py`` on torch tensors, linked against the installed torch and libreef_cuda.so."""
+    import sysconfig
+    import torch
+    out = os.path.join(PKG, "_decode.so")
+    srcs = sorted(glob.glob(os.path.join(CSRC, "torch", "*.cpp")))
+    deps = srcs + glob.glob(os.path.join(INCLUDE, "*.h"))
+    home = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    cmd = [_cxx()] + CXX_FLAGS + ["-I", INCLUDE, "-isystem", os.path.join(home, "include"), "-isystem",
+                                  os.path.join(home, "include", "torch", "csrc", "api", "include"), "-isystem", cuda, "-I",
+                                  sysconfig.get_paths()["include"], "-D_TORCH_VERSION_" + "".join(c if c.isalnum() else "_" for c in torch.__version__),
+                                  "-o", out] + srcs + \
+        ["-L", os.path.join(home, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L", PKG, "-lreef_cuda",
+         "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(home, "lib")]
+    _build(out, cmd, deps, verbose)
+    return out
+
+
 def build_all(verbose: bool = False):
-    return build_cuda(verbose), build_host(verbose)
+    cuda, host = build_cuda(verbose), build_host(verbose)
+    build_torch(verbose)
+    return cuda, host
 
 
 if __name__ == "__main__":

@@ -176,6 +176,7 @@ class Kernel:
         self._dims, smem, nargs = (C.c_uint32 * 6)(), C.c_uint32(), C.c_int()
         _check(lib.reef_kernel_geometry(self._h, self._dims, C.byref(smem), C.byref(nargs)), "reef_kernel_geometry")
         self._smem, self.num_args = smem.value, nargs.value
+        self.handle, self.dims, self.dyn_smem = self._h.value, list(self._dims), smem.value
         self._words, self._pointers = C.c_uint64 * nargs.value, C.c_void_p * nargs.value
         need = (C.c_size_t * max(16, nargs.value))()
         _check(lib.reef_kernel_arg_bytes(self._h, need, C.c_int(len(need))), "reef_kernel_arg_bytes")

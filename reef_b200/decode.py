@@ -18,12 +18,16 @@ while gradients are recorded.
 """
 from __future__ import annotations
 
+import threading
 from typing import NamedTuple, Optional
 
 import torch
 
-from .capi import OUT_OF_RANGE, FAIL, Kernel, ReefError
+from .capi import FAIL, OUT_OF_RANGE, Kernel, ReefError, cuda_lib
 from .resources import decoding
+
+cuda_lib()                      # (raises where the libraries are not built)
+from . import _decode           # noqa: E402
 
 _TYPES = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16"}
 
@@ -50,22 +54,28 @@ def page_state(rows: int, max_pages: int, tokens: int, *, fork: bool = False, de
 
 
 # ---- checks and launches -------------------------------------------------------------------------------------------------
+# A signature (types, devices, sizes, strides, options) is checked and resolved here, once; from then on _decode.call does everything.
+_TABLES, _APPEND, _ATTENTION, _BEAMS = range(4)
+_ready = set()      # devices whose kernels are set up
+_lock = threading.Lock()
+
+
 def _refuse(what: str, why: str):
     raise ReefError(OUT_OF_RANGE, what, why)
 
 
-_ready = set()      # devices whose kernels are set up
-_kernels = {}       # (operator, device, shapes, strides, types, options) -> kernels: a signature is checked once
-
-
-def _signature(*tensors):
-    return tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None for t in tensors)
+def _again(what, op, inputs, outputs, options):
+    """The call of a signature that has just been defined, or one that _decode.call has said no to."""
+    got = _decode.call(op, inputs, outputs, options)
+    if got.__class__ is not tuple:
+        _refuse(what, got if isinstance(got, str) else "arguments changed during the call")
+    return got
 
 
 def _inference(what, *tensors):
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 _refuse(what, "inputs require gradients and there is no backward pass (use torch.no_grad)")
 
 
@@ -111,50 +121,23 @@ def _resolve(what, device, names):
         kernels = [Kernel(n) for n in names]
     except ReefError as e:
         raise ReefError(OUT_OF_RANGE, what, str(e)) from None
-    if device not in _ready:
-        if torch.cuda.get_device_capability(device)[0] != 10:
-            raise ReefError(FAIL, what, f"{device} is not an sm_100 GPU")
-        with torch.cuda.device(device):
-            if torch.cuda.is_current_stream_capturing():
-                raise ReefError(FAIL, what, f"the first call on {device} has to be made outside a stream capture")
-            kernels[0].prepare([0] * kernels[0].num_args)
-        _ready.add(device)
+    with _lock:
+        if device not in _ready:
+            if torch.cuda.get_device_capability(device)[0] != 10:
+                raise ReefError(FAIL, what, f"{device} is not an sm_100 GPU")
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ReefError(FAIL, what, f"the first call on {device} has to be made outside a stream capture")
+                kernels[0].prepare([0] * kernels[0].num_args)
+            _ready.add(device)
     return kernels
 
 
-def _aligned(what, pointers):
-    for p in pointers:
-        if p & 15:
-            _refuse(what, "a tensor does not begin at a 16-byte boundary")
-
-
-def _apart(what, ins, outs):
-    """No output lies over an input or another output: a step reads one state and writes another, so that it can be run again."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in outs if t is not None]
-    for i, (a, b) in enumerate(spans):
-        for c, d in spans[:i]:
-            if a < d and c < b:
-                _refuse(what, "outputs lie over each other")
-    for t in ins:
-        if t is not None:
-            c = t.data_ptr()
-            d = c + t.numel() * t.element_size()
-            for a, b in spans:
-                if a < d and c < b:
-                    _refuse(what, "an output lies over an input")
-
-
-def _launch(device, launches):
-    """launches: (kernel, pointers), in order, on the device's current stream"""
-    if device.index == torch.cuda.current_device():
-        stream = torch.cuda.current_stream(device).cuda_stream
-        for kernel, pointers in launches:
-            kernel.launch(pointers, stream)
-    else:
-        with torch.cuda.device(device):
-            stream = torch.cuda.current_stream(device).cuda_stream
-            for kernel, pointers in launches:
-                kernel.launch(pointers, stream)
+def _define(op, inputs, outputs, options, kernels, args, allocate, workspace, aligned, apart):
+    """``args``: per kernel the tensors of its arguments, by position among inputs and outputs, -1 the workspace; ``allocate``: (input whose type
+    it has or -1 for int32, shape) per output; ``apart``: (position, positions that it must not lie over)."""
+    _decode.define(op, inputs, outputs, options, [(k.handle, k.dims, k.dyn_smem, a) for k, a in zip(kernels, args)], allocate, workspace, aligned,
+                   [x for i, others in apart for j in others for x in (i, j)])
 
 
 # ---- operators -------------------------------------------------------------------------------------------------------------
@@ -172,46 +155,45 @@ def page_tables(table, lens, new, *, pages: int, page_size: int, tokens: int, pa
     (``paged_attention`` leaves its tokens out).  Rows that cannot be served are refused by ``status`` and come out empty; the old state is
     still there, as ``out`` may not lie over it.
     """
-    what = "page_tables"
+    inputs, options = (table, lens, new, parent), (pages, page_size, tokens)
+    outputs = None if out is None else tuple(out[:5] if parent is None else out)
+    got = _decode.call(_TABLES, inputs, outputs, options)
+    if got.__class__ is not tuple:
+        got = _page_tables("page_tables", got, inputs, outputs, options)
+    return PageState(*got)
+
+
+def _page_tables(what, why, inputs, outputs, options):
+    if why is not None:
+        _refuse(what, why)
+    table, lens, new, parent = inputs
+    pages, page_size, tokens = options
     _tensors(what, table=table, lens=lens, new=new)
-    key = (what, _signature(table, lens, new, parent, *(out or ())), pages, page_size, tokens)
-    _inference(what, table, lens, new, parent)
-    kernels = _kernels.get(key)
-    if kernels is None:
-        if table.dim() != 2:
-            _refuse(what, "table is not [rows][max_pages]")
-        rows, device = table.shape[0], table.device
-        for name, v, hi in (("pages", pages, 1 << 19), ("page_size", page_size, 1024), ("tokens", tokens, 1 << 20)):
-            _whole(what, name, v, 1, hi)
-        if not 1 <= rows <= 1024 or table.shape[1] < 1:
-            _refuse(what, f"a table of {tuple(table.shape)}: 1 to 1024 rows of a page or more")
-        _want(what, "table", table, table.shape)
-        _want(what, "lens", lens, (rows,), device=device)
-        _want(what, "new", new, (rows,), device=device)
-        if parent is not None:
-            _want(what, "parent", parent, (rows,), device=device)
-        if out is not None:
-            if len(out) != 6:
-                _refuse(what, "out is not a PageState")
-            for name, t, shape in zip(PageState._fields, out, (table.shape, (rows,), (rows + 1,), (tokens, 4), (rows,), (rows, 4))):
-                if name != "fork" or parent is not None:
-                    _want(what, "out." + name, t, shape, device=device)
-        kernels = _resolve(what, device, [decoding.page_tables(rows, table.shape[1], page_size, pages, tokens, parent is not None)])
-        _kernels[key] = kernels
-    if out is None:
-        empty = lambda *shape: torch.empty(shape, dtype=torch.int32, device=table.device)    # noqa: E731
-        rows = table.shape[0]
-        out = PageState(torch.empty_like(table), empty(rows), empty(rows + 1), empty(tokens, 4), empty(rows),
-                        None if parent is None else empty(rows, 4))
-    elif parent is None and out[5] is not None:
-        out = PageState(*out[:5], None)
-    ins = [table, lens, new] + ([parent] if parent is not None else [])
-    outs = [t for t in out if t is not None]
-    _apart(what, ins, outs)
-    pointers = [t.data_ptr() for t in ins + outs]
-    _aligned(what, pointers[len(ins) + 3:len(ins) + 4] + pointers[len(ins) + 5:])
-    _launch(table.device, [(kernels[0], pointers)])
-    return out if isinstance(out, PageState) else PageState(*out)
+    _inference(what, *inputs)
+    if table.dim() != 2:
+        _refuse(what, "table is not [rows][max_pages]")
+    (rows, max_pages), device = table.shape, table.device
+    for name, v, hi in (("pages", pages, 1 << 19), ("page_size", page_size, 1024), ("tokens", tokens, 1 << 20)):
+        _whole(what, name, v, 1, hi)
+    if not 1 <= rows <= 1024 or max_pages < 1:
+        _refuse(what, f"a table of {tuple(table.shape)}: 1 to 1024 rows of a page or more")
+    _want(what, "table", table, table.shape)
+    _want(what, "lens", lens, (rows,), device=device)
+    _want(what, "new", new, (rows,), device=device)
+    if parent is not None:
+        _want(what, "parent", parent, (rows,), device=device)
+    shapes = [(rows, max_pages), (rows,), (rows + 1,), (tokens, 4), (rows,)] + ([(rows, 4)] if parent is not None else [])
+    if outputs is not None:
+        if len(outputs) != len(shapes):
+            _refuse(what, "out is not a PageState")
+        for name, t, shape in zip(PageState._fields, outputs, shapes):
+            _want(what, "out." + name, t, shape, device=device)
+    kernels = _resolve(what, device, [decoding.page_tables(rows, max_pages, page_size, pages, tokens, parent is not None)])
+    ins = [0, 1, 2] + ([3] if parent is not None else [])
+    outs = list(range(4, 4 + len(shapes)))
+    _define(_TABLES, inputs, outputs, options, kernels, [ins + outs], [(-1, s) for s in shapes], 0, [7] + outs[5:],
+            [(o, ins + outs[:n]) for n, o in enumerate(outs)])
+    return _again(what, _TABLES, inputs, outputs, options)
 
 
 def _cache(what, k_cache, v_cache, device):
@@ -233,37 +215,37 @@ def paged_append(k, v, tok, k_cache, v_cache, *, fork=None) -> None:
     in fp32, bf16 or fp16, rounded to nearest.  Tokens whose slot lies outside the cache are passed over.  Slots are distinct, and no
     token goes among those that a fork copies, as ``page_tables`` gives them; of two tokens with one slot either may be written, value by value.
     """
-    what = "paged_append"
+    inputs = (k, v, tok, k_cache, v_cache, fork)
+    got = _decode.call(_APPEND, inputs, None, ())
+    if got.__class__ is not tuple:
+        _paged_append("paged_append", got, inputs)
+
+
+def _paged_append(what, why, inputs):
+    if why is not None:
+        _refuse(what, why)
+    k, v, tok, k_cache, v_cache, fork = inputs
     _tensors(what, k=k, v=v, tok=tok, k_cache=k_cache, v_cache=v_cache)
-    key = (what, _signature(k, v, tok, k_cache, v_cache, fork))
-    _inference(what, k, v, k_cache, v_cache)
-    kernels = _kernels.get(key)
-    if kernels is None:
-        device = k.device
-        pages, kv, page, dim = _cache(what, k_cache, v_cache, device)
-        shape = (k.shape[0] if k.dim() else 0, kv, dim)
-        _want(what, "k", k, shape, torch.float32, device, dense=False)
-        _want(what, "v", v, shape, torch.float32, device, dense=False)
-        _want(what, "tok", tok, (shape[0], 4), device=device)
-        if not shape[0]:
-            _refuse(what, "no tokens")
-        if fork is not None:
-            if not isinstance(fork, torch.Tensor) or fork.dim() != 2 or not fork.shape[0]:
-                _refuse(what, "fork is not [rows][4]")
-            _want(what, "fork", fork, (fork.shape[0], 4), device=device)
-        strides = dict(ks=_token_stride(what, "k", k, kv, dim), vs=_token_stride(what, "v", v, kv, dim))
-        kernels = _resolve(what, device, [decoding.paged_append(shape[0], kv, dim, page, pages, _TYPES[k_cache.dtype],
-                                                                0 if fork is None else fork.shape[0], **strides)])
-        _kernels[key] = kernels
-    _apart(what, [tok, fork], [k_cache, v_cache])
-    ins = [k, v, tok] + ([fork] if fork is not None else [])
-    pointers = [t.data_ptr() for t in ins + [k_cache, v_cache]]
-    _aligned(what, pointers)
-    lo, hi = (min(pointers[-2:]), max(p + c.numel() * c.element_size() for p, c in zip(pointers[-2:], (k_cache, v_cache))))
-    for p, t in zip(pointers, (k, v)):
-        if lo < p + 4 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1] * t.shape[2]) and p < hi:
-            _refuse(what, "keys or values lie within the caches' memory")
-    _launch(k.device, [(kernels[0], pointers)])
+    _inference(what, *inputs)
+    device = k.device
+    pages, kv, page, dim = _cache(what, k_cache, v_cache, device)
+    shape = (k.shape[0] if k.dim() else 0, kv, dim)
+    _want(what, "k", k, shape, torch.float32, device, dense=False)
+    _want(what, "v", v, shape, torch.float32, device, dense=False)
+    _want(what, "tok", tok, (shape[0], 4), device=device)
+    if not shape[0]:
+        _refuse(what, "no tokens")
+    if fork is not None:
+        if not isinstance(fork, torch.Tensor) or fork.dim() != 2 or not fork.shape[0]:
+            _refuse(what, "fork is not [rows][4]")
+        _want(what, "fork", fork, (fork.shape[0], 4), device=device)
+    strides = dict(ks=_token_stride(what, "k", k, kv, dim), vs=_token_stride(what, "v", v, kv, dim))
+    kernels = _resolve(what, device, [decoding.paged_append(shape[0], kv, dim, page, pages, _TYPES[k_cache.dtype],
+                                                            0 if fork is None else fork.shape[0], **strides)])
+    copies = [] if fork is None else [5]
+    _define(_APPEND, inputs, None, (), kernels, [[0, 1, 2] + copies + [3, 4]], [], 0, [0, 1, 2, 3, 4] + copies,
+            [(3, [0, 1, 2, 4] + copies), (4, [0, 1, 2] + copies)])
+    _again(what, _APPEND, inputs, None, ())
 
 
 def paged_attention(q, k_cache, v_cache, table, tok, *, out=None):
@@ -275,43 +257,37 @@ def paged_attention(q, k_cache, v_cache, table, tok, *, out=None):
     output is zero.  Scores are scaled by 1 / sqrt(dim); sums and the softmax are fp32 whatever the cache's type.  Returns
     [tokens][heads][dim] fp32.
     """
-    what = "paged_attention"
+    inputs, outputs = (q, k_cache, v_cache, table, tok), None if out is None else (out,)
+    got = _decode.call(_ATTENTION, inputs, outputs, ())
+    if got.__class__ is not tuple:
+        got = _paged_attention("paged_attention", got, inputs, outputs)
+    return got[0]
+
+
+def _paged_attention(what, why, inputs, outputs):
+    if why is not None:
+        _refuse(what, why)
+    q, k_cache, v_cache, table, tok = inputs
     _tensors(what, q=q, k_cache=k_cache, v_cache=v_cache, table=table, tok=tok)
-    key = (what, _signature(q, k_cache, v_cache, table, tok, out))
-    _inference(what, q, k_cache, v_cache)
-    kernels = _kernels.get(key)
-    if kernels is None:
-        device = q.device
-        pages, kv, page, dim = _cache(what, k_cache, v_cache, device)
-        if q.dim() != 3 or not q.shape[0] or not q.shape[1] or q.shape[1] % kv:
-            _refuse(what, f"q of {tuple(q.shape)}: [tokens][heads][dim], heads a multiple of {kv}")
-        _want(what, "q", q, (q.shape[0], q.shape[1], dim), torch.float32, device, dense=False)
-        if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
-            _refuse(what, "table is not [rows][max_pages]")
-        _want(what, "table", table, table.shape, device=device)
-        _want(what, "tok", tok, (q.shape[0], 4), device=device)
-        if out is not None:
-            _want(what, "out", out, q.shape, torch.float32, device)
-        names = decoding.paged_attention(q.shape[0], table.shape[0], q.shape[1], kv, dim, page, table.shape[1], pages, _TYPES[k_cache.dtype],
-                                         qs=_token_stride(what, "q", q, q.shape[1], dim))
-        kernels = _resolve(what, device, names)
-        _kernels[key] = kernels
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    else:
-        _apart(what, [k_cache, v_cache, table, tok], [out])
-        a, b = q.data_ptr(), out.data_ptr()
-        if a < b + 4 * out.numel() and b < a + 4 * ((q.shape[0] - 1) * q.stride(0) + q.shape[1] * q.shape[2]):
-            _refuse(what, "an output lies over an input")
-    pointers = [q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), tok.data_ptr(), out.data_ptr()]
-    _aligned(what, pointers[:3] + pointers[4:])
-    if len(kernels) == 1:
-        _launch(q.device, [(kernels[0], pointers)])
-    else:
-        parts = torch.empty(kernels[0].arg_bytes[6], dtype=torch.uint8, device=q.device)
-        at = parts.data_ptr()
-        _launch(q.device, [(kernels[0], pointers + [at]), (kernels[1], [at, pointers[5]])])
-    return out
+    _inference(what, *inputs)
+    device = q.device
+    pages, kv, page, dim = _cache(what, k_cache, v_cache, device)
+    if q.dim() != 3 or not q.shape[0] or not q.shape[1] or q.shape[1] % kv:
+        _refuse(what, f"q of {tuple(q.shape)}: [tokens][heads][dim], heads a multiple of {kv}")
+    _want(what, "q", q, (q.shape[0], q.shape[1], dim), torch.float32, device, dense=False)
+    if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
+        _refuse(what, "table is not [rows][max_pages]")
+    _want(what, "table", table, table.shape, device=device)
+    _want(what, "tok", tok, (q.shape[0], 4), device=device)
+    if outputs is not None:
+        _want(what, "out", outputs[0], q.shape, torch.float32, device)
+    names = decoding.paged_attention(q.shape[0], table.shape[0], q.shape[1], kv, dim, page, table.shape[1], pages, _TYPES[k_cache.dtype],
+                                     qs=_token_stride(what, "q", q, q.shape[1], dim))
+    kernels = _resolve(what, device, names)
+    whole = [0, 1, 2, 3, 4, 5]
+    args, workspace = ([whole], 0) if len(kernels) == 1 else ([whole + [-1], [-1, 5]], kernels[0].arg_bytes[6])
+    _define(_ATTENTION, inputs, outputs, (), kernels, args, [(0, q.shape)], workspace, [0, 1, 2, 4, 5], [(5, [0, 1, 2, 3, 4])])
+    return _again(what, _ATTENTION, inputs, outputs, ())
 
 
 def beam_select(logits, score, live, *, beams: int, eos: int, start=None, out=None):
@@ -326,42 +302,42 @@ def beam_select(logits, score, live, *, beams: int, eos: int, start=None, out=No
     request has fewer candidates above -infinity than beams, the rest are token -1, parent -1, score -infinity, live 0: a row of logits with a
     NaN, an infinity or nothing but -infinity has none, nor has a beam whose score is not finite.
     """
-    what = "beam_select"
+    inputs, outputs, options = (logits, score, live, start), None if out is None else tuple(out), (beams, eos)
+    got = _decode.call(_BEAMS, inputs, outputs, options)
+    if got.__class__ is not tuple:
+        got = _beam_select("beam_select", got, inputs, outputs, options)
+    return got
+
+
+def _beam_select(what, why, inputs, outputs, options):
+    if why is not None:
+        _refuse(what, why)
+    logits, score, live, start = inputs
+    beams, eos = options
     _tensors(what, logits=logits, score=score, live=live)
-    key = (what, _signature(logits, score, live, start, *(out or ())), beams, eos)
-    _inference(what, logits, score)
-    kernels = _kernels.get(key)
-    if kernels is None:
-        device = logits.device
-        if logits.dim() != 2 or not logits.shape[0] or not logits.shape[1]:
-            _refuse(what, "logits are not [rows][vocab]")
-        _whole(what, "beams", beams, 1, 16)
-        _whole(what, "eos", eos, 0, logits.shape[1] - 1)
-        rows = score.shape[0] if score.dim() else 0
-        if not rows or rows % beams or (start is None and logits.shape[0] != rows):
-            _refuse(what, f"{rows} scores, {logits.shape[0]} rows of logits, {beams} beams to a request")
-        _want(what, "logits", logits, logits.shape, torch.float32, device)
-        _want(what, "score", score, (rows,), torch.float32, device)
-        _want(what, "live", live, (rows,), device=device)
-        if start is not None:
-            _want(what, "start", start, (rows + 1,), device=device)
-        if out is not None:
-            if len(out) != 4:
-                _refuse(what, "out is not (token, parent, score, live)")
-            for name, t, dtype in zip(("token", "parent", "score", "live"), out, (torch.int32, torch.int32, torch.float32, torch.int32)):
-                _want(what, "out " + name, t, (rows,), dtype, device)
-        kernels = _resolve(what, device, decoding.beam_select(rows // beams, beams, logits.shape[1], eos,
-                                                              None if start is None else logits.shape[0]))
-        _kernels[key] = kernels
-    if out is None:
-        block = torch.empty(4, score.shape[0], dtype=torch.int32, device=logits.device)
-        out = (block[0], block[1], block[2].view(torch.float32), block[3])
-    else:
-        _apart(what, [logits, score, live, start], out)
-    first = [] if start is None else [start.data_ptr()]
-    parts = torch.empty(kernels[0].arg_bytes[-1], dtype=torch.uint8, device=logits.device)
-    at, rows_at, live_at = parts.data_ptr(), logits.data_ptr(), live.data_ptr()
-    _aligned(what, [rows_at])
-    _launch(logits.device, [(kernels[0], [rows_at, live_at] + first + [at]),
-                            (kernels[1], [at, score.data_ptr(), live_at] + first + [t.data_ptr() for t in out])])
-    return tuple(out)
+    _inference(what, *inputs)
+    device = logits.device
+    if logits.dim() != 2 or not logits.shape[0] or not logits.shape[1]:
+        _refuse(what, "logits are not [rows][vocab]")
+    _whole(what, "beams", beams, 1, 16)
+    _whole(what, "eos", eos, 0, logits.shape[1] - 1)
+    rows = score.shape[0] if score.dim() else 0
+    if not rows or rows % beams or (start is None and logits.shape[0] != rows):
+        _refuse(what, f"{rows} scores, {logits.shape[0]} rows of logits, {beams} beams to a request")
+    _want(what, "logits", logits, logits.shape, torch.float32, device)
+    _want(what, "score", score, (rows,), torch.float32, device)
+    _want(what, "live", live, (rows,), device=device)
+    if start is not None:
+        _want(what, "start", start, (rows + 1,), device=device)
+    if outputs is not None:
+        if len(outputs) != 4:
+            _refuse(what, "out is not (token, parent, score, live)")
+        for name, t, dtype in zip(("token", "parent", "score", "live"), outputs, (torch.int32, torch.int32, torch.float32, torch.int32)):
+            _want(what, "out " + name, t, (rows,), dtype, device)
+    kernels = _resolve(what, device, decoding.beam_select(rows // beams, beams, logits.shape[1], eos, None if start is None else logits.shape[0]))
+    first = [] if start is None else [3]
+    ins, outs = [0, 1, 2] + first, [4, 5, 6, 7]
+    _define(_BEAMS, inputs, outputs, options, kernels, [[0, 2] + first + [-1], [-1, 1, 2] + first + outs],
+            [(-1, (rows,)), (-1, (rows,)), (1, (rows,)), (-1, (rows,))], kernels[0].arg_bytes[-1], [0],
+            [(o, ins + outs[:n]) for n, o in enumerate(outs)])
+    return _again(what, _BEAMS, inputs, outputs, options)
