@@ -45,11 +45,16 @@ struct PagedFns {
     }
 };
 template <int D>
+static const void* paged_fp32_eight() { return (const void*)k_paged_attention<PagedSimt<float, D, 8>, 2>; }
+template <>
+const void* paged_fp32_eight<256>() { return nullptr; }
+template <int D>
 struct PagedFns<float, D> {
     static const void* of(int gb) {
         return gb == 1 ? (const void*)k_paged_attention<PagedSimt<float, D, 1>, 2>
              : gb == 2 ? (const void*)k_paged_attention<PagedSimt<float, D, 2>, 2>
-             : gb == 4 ? (const void*)k_paged_attention<PagedSimt<float, D, 4>, 2> : nullptr;
+             : gb == 4 ? (const void*)k_paged_attention<PagedSimt<float, D, 4>, 2>
+             : gb == 8 ? paged_fp32_eight<D>() : nullptr;
     }
 };
 template <class C>

@@ -93,8 +93,12 @@ struct PagedRing {
 };
 
 // ---- fp32 instructions ----------------------------------------------------------------------------------------------------
-// A lane holds 16 bytes of a key (4 or 8 dimensions; 8 of 256 in fp32 take two pieces), the lanes of a key meet in shuffles; every
-// group of lanes keeps its own maximum and sums until the end of its range.
+// A lane holds 16 bytes of a key (4 or 8 dimensions; 8 of 256 in fp32 take two pieces).  The lanes of a key bring their parts of the scores
+// together by halves, so that in the end every score stands in a lane of its own: half as many shuffles as sums over all lanes, and one
+// exponential for all scores of a step instead of one each.  Every group of lanes keeps its own maximum and sums until the end of its range.
+__host__ __device__ constexpr int paged_log2(int x) { return x <= 1 ? 0 : 1 + paged_log2(x / 2); }
+// keys of a lane in a step: its scores fill at most the lanes of a key, and registers
+__host__ __device__ constexpr int paged_simt_keys(int pieces, int gb) { return (gb >= 8 ? 2 : 4) / pieces; }
 template <class C, int D, int GB_, int RING_ = kPagedSimtRing>
 struct PagedSimt {
     static constexpr int GB = GB_, DIM = D, RING = RING_;
@@ -103,35 +107,54 @@ struct PagedSimt {
     static constexpr int LD = D / (VEC * LPT);                          // pieces of a lane and key
     static constexpr int E = VEC * LD;                                  // dimensions of a lane
     static constexpr int TPI = 32 / LPT;                                // keys of a warp's piece
-    static constexpr int U = 4 / LD;                                    // keys of a lane in a step
+    static constexpr int U = paged_simt_keys(LD, GB);                   // keys of a lane in a step
     static constexpr int UNIT = TPI * U;                                // keys of a step
-    static constexpr int STAGE = U * LD * 512, SCRATCH = RING * STAGE;
+    static constexpr int STAGE = U * LD * 512, SCRATCH = RING * STAGE > GB * paged_stride(D) * 4 ? RING * STAGE : GB * paged_stride(D) * 4;
+    static constexpr int N = U * GB, SPREAD = LPT / N;                  // scores of a step and key lane; lanes that hold the same one
+    static_assert(N <= LPT, "a lane to a score");
     float2 q[GB][E / 2], o[GB][E / 2];
-    float m[GB], l[GB];
+    float m, l;                                                          // of this lane's head
 
     static __device__ __forceinline__ int dim(int lane, int e) { return (e / VEC) * (LPT * VEC) + (lane % LPT) * VEC + e % VEC; }
+    // the lane (of this lane's group) that has the score of its u-th key and head j
+    static __device__ __forceinline__ int holder(int lane, int u, int j) { return lane / LPT * LPT + (u * GB + j) * SPREAD; }
 
     // false: the preempt flag went up
     __device__ __forceinline__ bool run(const PagedRow& r, char* scratch, const int* flag) {
-        const int lane = threadIdx.x & 31, sub = lane / LPT;
+        const int lane = threadIdx.x & 31, sub = lane / LPT, mine_u = lane % LPT / SPREAD / GB;
         const C* kc = (const C*)r.k + (lane % LPT) * VEC;
         const C* vc = (const C*)r.v + (lane % LPT) * VEC;
         PagedRing<RING, STAGE> ring(scratch + lane * 16);        // (a lane's pieces are its own)
+        // a step's keys lie in one page where the pages hold whole steps (steps begin at multiples of their size)
+        const bool one_page = r.ps % UNIT == 0;
         int at[U], id[U], pos_in = r.begin;
 #pragma unroll
-        for (int u = 0; u < U; u++) id[u] = r.page(r.begin + u * TPI + sub);
+        for (int u = 0; u < U; u++)
+            if (u == 0 || !one_page) id[u] = r.page(r.begin + u * TPI + sub);
         unsigned there = 0;             // a bit per key of a lane, four to a step, the newest lowest
         auto issue_k = [&]() {
             const uint32_t to = ring.put();
             there <<= 4;
             if (pos_in < r.end) {
+                if (one_page) {
+                    at[0] = r.place(pos_in + sub, __shfl_sync(0xffffffffu, id[0], 0));   // (the first key is there)
+#pragma unroll
+                    for (int u = 1; u < U; u++) at[u] = at[0] >= 0 && pos_in + u * TPI + sub < r.end ? at[0] + u * TPI : -1;
+                    if (pos_in + sub >= r.end) at[0] = -1;
+                    id[0] = r.page(pos_in + UNIT);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        at[u] = r.place(pos_in + u * TPI + sub, id[u]);
+                        id[u] = r.page(pos_in + UNIT + u * TPI + sub);
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    at[u] = r.place(pos_in + u * TPI + sub, id[u]);
-                    id[u] = r.page(pos_in + UNIT + u * TPI + sub);
                     there |= (at[u] >= 0 ? 1u : 0u) << u;
+                    const C* from = kc + (size_t)max(at[u], 0) * D;
 #pragma unroll
-                    for (int i = 0; i < LD; i++) copy16(to + (u * LD + i) * 512, kc + (size_t)max(at[u], 0) * D + i * LPT * VEC, at[u] >= 0);
+                    for (int i = 0; i < LD; i++) copy16(to + (u * LD + i) * 512, from + i * LPT * VEC, at[u] >= 0);
                 }
             }
             copy_commit();
@@ -140,9 +163,11 @@ struct PagedSimt {
             const uint32_t to = ring.put();
             if (pos_in < r.end) {
 #pragma unroll
-                for (int u = 0; u < U; u++)
+                for (int u = 0; u < U; u++) {
+                    const C* from = vc + (size_t)max(at[u], 0) * D;
 #pragma unroll
-                    for (int i = 0; i < LD; i++) copy16(to + (u * LD + i) * 512, vc + (size_t)max(at[u], 0) * D + i * LPT * VEC, at[u] >= 0);
+                    for (int i = 0; i < LD; i++) copy16(to + (u * LD + i) * 512, from + i * LPT * VEC, at[u] >= 0);
+                }
             }
             copy_commit();
             pos_in += UNIT;
@@ -166,9 +191,9 @@ struct PagedSimt {
             }
 #pragma unroll
             for (int e = 0; e < E / 2; e++) o[j][e] = make_float2(0.f, 0.f);
-            m[j] = -INFINITY;
-            l[j] = 0.f;
         }
+        m = -INFINITY;
+        l = 0.f;
         int up = 0, steps = 0;
         bool stopped = false;
 #pragma unroll 1
@@ -181,14 +206,7 @@ struct PagedSimt {
                 up = ld_flag(flag);
             }
             uint32_t from = ring.take();
-            uint4 x[U][LD];
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int i = 0; i < LD; i++) x[u][i] = read16(from + (u * LD + i) * 512);
-            issue_v();
-            const unsigned now = there >> (RING - 1) / 2 * 4;            // (as many steps are ahead of this one)
-            float s[U][GB];
+            float s[N];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 float2 sum[GB];
@@ -197,91 +215,104 @@ struct PagedSimt {
 #pragma unroll
                 for (int i = 0; i < LD; i++) {
                     float2 y[VEC / 2];
-                    unpack(x[u][i], y, C());
+                    unpack(read16(from + (u * LD + i) * 512), y, C());
 #pragma unroll
                     for (int e = 0; e < VEC / 2; e++)
 #pragma unroll
                         for (int j = 0; j < GB; j++) sum[j] = fma2(q[j][i * VEC / 2 + e], y[e], sum[j]);
                 }
 #pragma unroll
-                for (int j = 0; j < GB; j++) s[u][j] = sum[j].x + sum[j].y;
+                for (int j = 0; j < GB; j++) s[u * GB + j] = sum[j].x + sum[j].y;
             }
+            issue_v();
+            const unsigned now = there >> (RING - 1) / 2 * 4;            // (as many steps are ahead of this one)
+            // a lane keeps the half of the scores that its bit names and gives the other one away
 #pragma unroll
-            for (int w = LPT / 2; w > 0; w >>= 1)
+            for (int w = LPT / 2, n = N; w > 0; w >>= 1) {
+                if (n > 1) {
+                    n >>= 1;
+                    const bool upper = lane & w;
 #pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int j = 0; j < GB; j++) s[u][j] += __shfl_xor_sync(0xffffffffu, s[u][j], w);
-#pragma unroll
-            for (int j = 0; j < GB; j++) {
-                float top = m[j];
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (!(now >> u & 1)) s[u][j] = -INFINITY;
-                    top = fmaxf(top, s[u][j]);
-                }
-                if (top != m[j]) {
-                    const float by = exp2_fast(m[j] - top);
-                    l[j] *= by;
-#pragma unroll
-                    for (int e = 0; e < E / 2; e++) o[j][e] = make_float2(o[j][e].x * by, o[j][e].y * by);
-                    m[j] = top;
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    s[u][j] = s[u][j] == -INFINITY ? 0.f : exp2_fast(s[u][j] - top);
-                    l[j] += s[u][j];
+                    for (int i = 0; i < n; i++) {
+                        const float give = upper ? s[i] : s[n + i];
+                        s[i] = (upper ? s[n + i] : s[i]) + __shfl_xor_sync(0xffffffffu, give, w);
+                    }
+                } else {
+                    s[0] += __shfl_xor_sync(0xffffffffu, s[0], w);
                 }
             }
+            const float score = now >> mine_u & 1 ? s[0] : -INFINITY;
+            float top = fmaxf(m, score);
+#pragma unroll
+            for (int w = LPT / U; w < LPT; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            if (__any_sync(0xffffffffu, top != m)) {
+                const float by = top == m ? 1.f : exp2_fast(m - top);
+                l *= by;
+#pragma unroll
+                for (int j = 0; j < GB; j++) {
+                    const float b = __shfl_sync(0xffffffffu, by, holder(lane, 0, j));
+#pragma unroll
+                    for (int e = 0; e < E / 2; e++) o[j][e] = make_float2(o[j][e].x * b, o[j][e].y * b);
+                }
+                m = top;
+            }
+            const float p = score == -INFINITY ? 0.f : exp2_fast(score - top);
+            l += p;
             from = ring.take();
 #pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int i = 0; i < LD; i++) x[u][i] = read16(from + (u * LD + i) * 512);
-            issue_k();
-#pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++) {
+                float2 y[E / 2];
 #pragma unroll
                 for (int i = 0; i < LD; i++) {
-                    float2 y[VEC / 2];
-                    unpack(x[u][i], y, C());
+                    float2 z[VEC / 2];
+                    unpack(read16(from + (u * LD + i) * 512), z, C());
 #pragma unroll
-                    for (int e = 0; e < VEC / 2; e++)
-#pragma unroll
-                        for (int j = 0; j < GB; j++) o[j][i * VEC / 2 + e] = fma2(make_float2(s[u][j], s[u][j]), y[e], o[j][i * VEC / 2 + e]);
+                    for (int e = 0; e < VEC / 2; e++) y[i * VEC / 2 + e] = z[e];
                 }
+#pragma unroll
+                for (int j = 0; j < GB; j++) {
+                    const float b = __shfl_sync(0xffffffffu, p, holder(lane, u, j));
+#pragma unroll
+                    for (int e = 0; e < E / 2; e++) o[j][e] = fma2(make_float2(b, b), y[e], o[j][e]);
+                }
+            }
+            issue_k();
         }
         copy_wait<0>();
         if (stopped) return false;
-        // the groups of lanes meet
+        // the keys of a lane group's lanes, then the groups
 #pragma unroll
-        for (int w = LPT; w < 32; w <<= 1)
+        for (int w = LPT / U; w < LPT; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+#pragma unroll
+        for (int w = LPT; w < 32; w <<= 1) {
+            const float mo = __shfl_xor_sync(0xffffffffu, m, w), top = fmaxf(m, mo);
+            const float a = m == top ? 1.f : exp2_fast(m - top), b = mo == top ? 1.f : exp2_fast(mo - top);
+            l = l * a + __shfl_xor_sync(0xffffffffu, l, w) * b;
+            m = top;
 #pragma unroll
             for (int j = 0; j < GB; j++) {
-                const float mo = __shfl_xor_sync(0xffffffffu, m[j], w), top = fmaxf(m[j], mo);
-                const float a = m[j] == top ? 1.f : exp2_fast(m[j] - top), b = mo == top ? 1.f : exp2_fast(mo - top);
-                l[j] = l[j] * a + __shfl_xor_sync(0xffffffffu, l[j], w) * b;
+                const float aj = __shfl_sync(0xffffffffu, a, holder(lane, 0, j)), bj = __shfl_sync(0xffffffffu, b, holder(lane, 0, j));
 #pragma unroll
                 for (int e = 0; e < E / 2; e++) {
-                    o[j][e].x = o[j][e].x * a + __shfl_xor_sync(0xffffffffu, o[j][e].x, w) * b;
-                    o[j][e].y = o[j][e].y * a + __shfl_xor_sync(0xffffffffu, o[j][e].y, w) * b;
+                    o[j][e].x = o[j][e].x * aj + __shfl_xor_sync(0xffffffffu, o[j][e].x, w) * bj;
+                    o[j][e].y = o[j][e].y * aj + __shfl_xor_sync(0xffffffffu, o[j][e].y, w) * bj;
                 }
-                m[j] = top;
             }
+        }
         return true;
     }
     __device__ __forceinline__ void store(const PagedRow& r, float* at, int stride, bool finished) const {
         const int lane = threadIdx.x & 31;
-        if (lane >= LPT) return;
 #pragma unroll
         for (int j = 0; j < GB; j++) {
-            if (j >= r.heads) break;
-            const float by = !finished ? 1.f : l[j] == 0.f ? 0.f : 1.f / l[j];
+            const float lj = __shfl_sync(0xffffffffu, l, holder(0, 0, j)), mj = __shfl_sync(0xffffffffu, m, holder(0, 0, j));
+            if (j >= r.heads || lane >= LPT) continue;
+            const float by = !finished ? 1.f : lj == 0.f ? 0.f : 1.f / lj;
 #pragma unroll
             for (int e = 0; e < E; e += 4)
                 *reinterpret_cast<float4*>(at + j * stride + dim(lane, e)) =
                     make_float4(o[j][e / 2].x * by, o[j][e / 2].y * by, o[j][e / 2 + 1].x * by, o[j][e / 2 + 1].y * by);
-            if (!finished && lane == 0) *reinterpret_cast<float2*>(at + j * stride + D) = make_float2(m[j], l[j]);
+            if (!finished && lane == 0) *reinterpret_cast<float2*>(at + j * stride + D) = make_float2(mj, lj);
         }
     }
 };
@@ -744,9 +775,13 @@ __device__ __forceinline__ bool paged_attention_body(const KTask& t, int vb, uns
             const int j = i / (E::DIM / 4), c = (i - j * (E::DIM / 4)) * 4;
             float top = -INFINITY, sum = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (unsigned x = slots; x; x &= x - 1) top = fmaxf(top, slot(__ffs(x) - 1)[j * stride + E::DIM]);
-            for (unsigned x = slots; x; x &= x - 1) {
-                const float* from = slot(__ffs(x) - 1) + j * stride;
+#pragma unroll
+            for (int x = 0; x < 16; x++)
+                if (slots >> x & 1) top = fmaxf(top, slot(x)[j * stride + E::DIM]);
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                if (!(slots >> x & 1)) continue;
+                const float* from = slot(x) + j * stride;
                 const float2 ml = *reinterpret_cast<const float2*>(from + E::DIM);
                 const float4 y = *reinterpret_cast<const float4*>(from + c);
                 const float by = ml.x == top ? 1.f : exp2_fast(ml.x - top);
@@ -768,15 +803,19 @@ __device__ __forceinline__ bool paged_attention_body(const KTask& t, int vb, uns
 
 // ---- shapes ---------------------------------------------------------------------------------------------------------------
 // Tensor cores from three query heads to a 16-bit key head on.
-__host__ inline int paged_heads_of_a_pass(int kt, int d, int group) { return group <= 2 ? group : kt == KT_FP32 || group <= 4 ? 4 : 8; }
-__host__ inline bool paged_mma(const PagedP& p) { return p.kt != KT_FP32 && p.gb > 2; }
-__host__ inline int paged_unit(const PagedP& p) {          // keys of a warp's step (UNIT above)
-    if (paged_mma(p)) return 16;
-    const int vec = p.kt == KT_FP32 ? 4 : 8, lanes = p.d / vec > 32 ? 32 : p.d / vec;
-    return 32 / lanes * (p.d > 32 * vec ? 2 : 4);
+__host__ inline int paged_heads_of_a_pass(int kt, int d, int group) {
+    return group <= 2 ? group : group <= 4 || (kt == KT_FP32 && d == 256) ? 4 : 8;
 }
+__host__ inline bool paged_mma(const PagedP& p) { return p.kt != KT_FP32 && p.gb > 2; }
+struct PagedSimtShape { int unit, scratch; };
+__host__ inline PagedSimtShape paged_simt_shape(const PagedP& p) {      // UNIT and SCRATCH of PagedSimt
+    const int vec = p.kt == KT_FP32 ? 4 : 8, lanes = p.d / vec > 32 ? 32 : p.d / vec, pieces = p.d / (vec * lanes), keys = paged_simt_keys(pieces, p.gb);
+    const int ring = kPagedSimtRing * keys * pieces * 512, slot = p.gb * paged_stride(p.d) * 4;
+    return {32 / lanes * keys, ring > slot ? ring : slot};
+}
+__host__ inline int paged_unit(const PagedP& p) { return paged_mma(p) ? 16 : paged_simt_shape(p).unit; }      // keys of a warp's step
 __host__ inline int paged_attention_smem(const PagedP& p) {
-    return (int)((sizeof(PagedSlots) + 15) & ~15) + 8 * (paged_mma(p) ? paged_mma_scratch(p.d, p.gb) : kPagedSimtRing * 2048);
+    return (int)((sizeof(PagedSlots) + 15) & ~15) + 8 * (paged_mma(p) ? paged_mma_scratch(p.d, p.gb) : paged_simt_shape(p).scratch);
 }
 __host__ inline int paged_blocks_per_sm(const PagedP& p) { return paged_mma(p) && p.d == 256 ? 1 : 2; }
 __host__ inline size_t paged_parts_bytes(const PagedP& p, int blocks) {
