@@ -228,12 +228,13 @@ struct PagedSimt {
             const unsigned now = there >> (RING - 1) / 2 * 4;            // (as many steps are ahead of this one)
             // a lane keeps the half of the scores that its bit names and gives the other one away
 #pragma unroll
-            for (int w = LPT / 2, n = N; w > 0; w >>= 1) {
-                if (n > 1) {
-                    n >>= 1;
+            for (int level = 1; level <= paged_log2(LPT); level++) {
+                const int w = LPT >> level, n = N >> level;
+                if (n > 0) {
                     const bool upper = lane & w;
 #pragma unroll
-                    for (int i = 0; i < n; i++) {
+                    for (int i = 0; i < N / 2; i++) {
+                        if (i >= n) break;
                         const float give = upper ? s[i] : s[n + i];
                         s[i] = (upper ? s[n + i] : s[i]) + __shfl_xor_sync(0xffffffffu, give, w);
                     }
@@ -802,6 +803,7 @@ __device__ __forceinline__ bool paged_attention_body(const KTask& t, int vb, uns
 }
 
 // ---- shapes ---------------------------------------------------------------------------------------------------------------
+constexpr int kSmsPlanned = 148;                           // launch geometry is planned without a GPU
 // Tensor cores from three query heads to a 16-bit key head on.
 __host__ inline int paged_heads_of_a_pass(int kt, int d, int group) {
     return group <= 2 ? group : group <= 4 || (kt == KT_FP32 && d == 256) ? 4 : 8;
@@ -818,17 +820,23 @@ __host__ inline int paged_attention_smem(const PagedP& p) {
     return (int)((sizeof(PagedSlots) + 15) & ~15) + 8 * (paged_mma(p) ? paged_mma_scratch(p.d, p.gb) : paged_simt_shape(p).scratch);
 }
 __host__ inline int paged_blocks_per_sm(const PagedP& p) { return paged_mma(p) && p.d == 256 ? 1 : 2; }
+// Blocks of the form with parts: what the SMs hold at once, fewer where the longest rows would not give every warp its least work.  (SMs do
+// not get the same share of the memory's bandwidth: of 148 equal shares of 860 MB one was through after 107 us and one after 147.  Two or
+// three times as many blocks, to be taken by whichever SM is free, brought 157 to 152 us, and cost more in further parts and their join.)
+__host__ inline int paged_parts_blocks(const PagedP& p, long long units) {
+    const long long want = (units + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits), slots = (long long)paged_blocks_per_sm(p) * kSmsPlanned;
+    return (int)(want < slots ? want : slots);
+}
 __host__ inline size_t paged_parts_bytes(const PagedP& p, int blocks) {
     return ((size_t)2 * ((blocks + 1) & ~1) + (size_t)blocks * kPagedSlotsOfBlock * p.gb * paged_stride(p.d)) * 4;
 }
 
-constexpr int kSmsPlanned = 148;                           // launch geometry is planned without a GPU
 // ---- join -----------------------------------------------------------------------------------------------------------------
 // args: parts, out.  A pass that block b left unfinished: its part, then those of the blocks behind it that lie in the same pass, added in
 // their order.  Few parts: a warp to a head of a pass.  Many (a long row): a block to 32 dimensions of a head, the parts divided
 // among groups of eight lanes, the groups added in their order.
 constexpr int kJoinFew = 16;
-__host__ __device__ inline int paged_join_blocks(int blocks, int gb) { return min((blocks * gb + 7) / 8, kSmsPlanned); }
+__host__ __device__ inline int paged_join_blocks(int blocks, int gb) { return min((blocks * gb + 7) / 8, 2 * kSmsPlanned); }
 __device__ __forceinline__ bool body_paged_join(const KTask& t, int vb, unsigned char* smem, const int*) {
     const PagedP& p = t.p.paged;
     const int blocks = p.split, gb = p.gb, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.d;

@@ -176,8 +176,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
     const long long passes = (long long)p.tokens * p.kvh * p.subs;
     const int units = ceil_div(p.mp * p.ps, paged_unit(p));
     if (passes * units > 0x70000000LL) return false;
-    // With parts: what the SMs hold at once, fewer where the longest rows would not give every warp its least work.
-    const int blocks = (int)std::min<long long>(paged_blocks_per_sm(p) * kSmsPlanned, (passes * units + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits));
+    const int blocks = paged_parts_blocks(p, passes * units);
     if (join) {
         p.split = blocks;
         t.family = F_PAGED_JOIN;
