@@ -376,9 +376,10 @@ static int build_spec(const std::string& name, KernelSpec* s) {
         int sN, h, vocab;
         if (!a.need("s", &sN) || !a.need("h", &h) || !a.need("vocab", &vocab) || (h & 3)) goto bad;
         t.p.raw[0] = sN; t.p.raw[1] = h; t.p.raw[2] = vocab;
+        if (!maybe_between(a, "npos", 1, 1 << 24, 0, &t.p.raw[3])) goto bad;
         t.family = F_EMBEDDING;
         t.nblocks = ceil_div(sN * (h / 4), kThreads * 4);
-        s->nargs = 4;
+        s->nargs = t.p.raw[3] ? 5 : 4;
         s->bytes = 4.0 * 3.0 * sN * h + 8.0 * sN;
         return REEF_SUCC;
     }
@@ -613,7 +614,8 @@ static void fill_arg_bytes(KernelSpec* s) {
             break;
         case F_EMBEDDING: {
             const double sN = t.p.raw[0], h = t.p.raw[1], vocab = t.p.raw[2];
-            b[0] = f4(sN * h); b[1] = f4(vocab * h); b[2] = (size_t)sN * 8; b[3] = f4(sN * h);
+            b[0] = f4(sN * h); b[1] = f4(vocab * h); b[2] = (size_t)sN * 8; b[3] = f4((t.p.raw[3] ? (double)t.p.raw[3] : sN) * h);
+            if (t.p.raw[3]) b[4] = f4(4.0 * sN);
             break;
         }
         case F_LAYERNORM: {

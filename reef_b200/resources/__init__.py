@@ -12,6 +12,7 @@ import os
 from .graph import Graph, kname, parse_kname, read_param_file, write_param_file  # noqa: F401
 from .mocked import build_mocked_kernel
 from .bert import build_bert
+from .decoder import build_decoder
 from .densenet import build_densenet
 from .inception import build_inception_v3
 from .resnet import build_resnet
@@ -30,6 +31,9 @@ _BUILDERS = {
     "bert_base": lambda **kw: build_bert(**kw),
     "bert_tiny": lambda **kw: build_bert(name="bert_tiny", layers=2, hidden=128, heads=2, ffn=256, vocab=1000, seq=48,
                                          seed=5048, **kw),
+    "decoder": lambda **kw: build_decoder(**kw),
+    "decoder_tiny": lambda **kw: build_decoder(**{**dict(name="decoder_tiny", layers=2, hidden=256, heads=4, kv_heads=2, ffn=512, vocab=1000,
+                                                         requests=2, beams=3, tokens=40, page_size=8, max_pages=12, pages=80, seed=7048), **kw}),
     "inception_v3": lambda **kw: build_inception_v3(**kw),
     "inception_v3_139": lambda **kw: build_inception_v3(name="inception_v3_139", image=139, seed=4139, **kw),
     "vgg16": lambda **kw: build_vgg16(**kw),
