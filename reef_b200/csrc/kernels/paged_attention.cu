@@ -44,17 +44,24 @@ struct PagedFns {
              : gb == 8 ? (const void*)k_paged_attention<PagedMma<C, D, 8>, D == 256 ? 1 : 2> : nullptr;
     }
 };
-template <int D>
-static const void* paged_fp32_eight() { return (const void*)k_paged_attention<PagedSimt<float, D, 8>, 2>; }
-template <>
-const void* paged_fp32_eight<256>() { return nullptr; }
+template <int D, int GB>
+static const void* paged_fp32() {
+    if constexpr (D == 256 && GB > 4) return nullptr;
+    else return (const void*)k_paged_attention<PagedSimt<float, D, GB>, 2>;
+}
 template <int D>
 struct PagedFns<float, D> {
     static const void* of(int gb) {
-        return gb == 1 ? (const void*)k_paged_attention<PagedSimt<float, D, 1>, 2>
-             : gb == 2 ? (const void*)k_paged_attention<PagedSimt<float, D, 2>, 2>
-             : gb == 4 ? (const void*)k_paged_attention<PagedSimt<float, D, 4>, 2>
-             : gb == 8 ? paged_fp32_eight<D>() : nullptr;
+        switch (gb) {
+            case 1: return paged_fp32<D, 1>();
+            case 2: return paged_fp32<D, 2>();
+            case 3: return paged_fp32<D, 3>();
+            case 4: return paged_fp32<D, 4>();
+            case 5: return paged_fp32<D, 5>();
+            case 6: return paged_fp32<D, 6>();
+            case 8: return paged_fp32<D, 8>();
+            default: return nullptr;
+        }
     }
 };
 template <class C>
@@ -72,7 +79,7 @@ int paged_prepare_device() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16 || done[dev]) return REEF_SUCC;
     for (int kt = KT_FP32; kt <= KT_FP16; kt++)
         for (int d = 64; d <= 256; d *= 2)
-            for (int gb = 1; gb <= 8; gb *= 2) {
+            for (int gb = 1; gb <= 8; gb++) {
                 PagedP p;
                 p.kt = kt; p.d = d; p.gb = gb;
                 const void* fn = paged_fn(p);

@@ -97,8 +97,12 @@ struct PagedRing {
 // together by halves, so that in the end every score stands in a lane of its own: half as many shuffles as sums over all lanes, and one
 // exponential for all scores of a step instead of one each.  Every group of lanes keeps its own maximum and sums until the end of its range.
 __host__ __device__ constexpr int paged_log2(int x) { return x <= 1 ? 0 : 1 + paged_log2(x / 2); }
+__host__ __device__ constexpr int paged_pow2(int x) { return x <= 1 ? 1 : 2 * paged_pow2((x + 1) / 2); }
 // keys of a lane in a step: its scores fill at most the lanes of a key, and registers
-__host__ __device__ constexpr int paged_simt_keys(int pieces, int gb) { return (gb >= 8 ? 2 : 4) / pieces; }
+__host__ __device__ constexpr int paged_simt_keys(int pieces, int lanes, int gb) {
+    const int most = (gb > 6 ? 2 : 4) / pieces, room = lanes / paged_pow2(gb);
+    return most < room ? most : room;
+}
 template <class C, int D, int GB_, int RING_ = kPagedSimtRing>
 struct PagedSimt {
     static constexpr int GB = GB_, DIM = D, RING = RING_;
@@ -107,21 +111,21 @@ struct PagedSimt {
     static constexpr int LD = D / (VEC * LPT);                          // pieces of a lane and key
     static constexpr int E = VEC * LD;                                  // dimensions of a lane
     static constexpr int TPI = 32 / LPT;                                // keys of a warp's piece
-    static constexpr int U = paged_simt_keys(LD, GB);                   // keys of a lane in a step
+    static constexpr int U = paged_simt_keys(LD, LPT, GB);              // keys of a lane in a step
     static constexpr int UNIT = TPI * U;                                // keys of a step
     static constexpr int STAGE = U * LD * 512, SCRATCH = RING * STAGE > GB * paged_stride(D) * 4 ? RING * STAGE : GB * paged_stride(D) * 4;
-    static constexpr int N = U * GB, SPREAD = LPT / N;                  // scores of a step and key lane; lanes that hold the same one
+    static constexpr int G2 = paged_pow2(GB), N = U * G2, SPREAD = LPT / N;     // scores of a step and key lane; lanes that hold the same one
     static_assert(N <= LPT, "a lane to a score");
     float2 q[GB][E / 2], o[GB][E / 2];
     float m, l;                                                          // of this lane's head
 
     static __device__ __forceinline__ int dim(int lane, int e) { return (e / VEC) * (LPT * VEC) + (lane % LPT) * VEC + e % VEC; }
     // the lane (of this lane's group) that has the score of its u-th key and head j
-    static __device__ __forceinline__ int holder(int lane, int u, int j) { return lane / LPT * LPT + (u * GB + j) * SPREAD; }
+    static __device__ __forceinline__ int holder(int lane, int u, int j) { return lane / LPT * LPT + (u * G2 + j) * SPREAD; }
 
     // false: the preempt flag went up
     __device__ __forceinline__ bool run(const PagedRow& r, char* scratch, const int* flag) {
-        const int lane = threadIdx.x & 31, sub = lane / LPT, mine_u = lane % LPT / SPREAD / GB;
+        const int lane = threadIdx.x & 31, sub = lane / LPT, mine_u = lane % LPT / SPREAD / G2;
         const C* kc = (const C*)r.k + (lane % LPT) * VEC;
         const C* vc = (const C*)r.v + (lane % LPT) * VEC;
         PagedRing<RING, STAGE> ring(scratch + lane * 16);        // (a lane's pieces are its own)
@@ -222,7 +226,7 @@ struct PagedSimt {
                         for (int j = 0; j < GB; j++) sum[j] = fma2(q[j][i * VEC / 2 + e], y[e], sum[j]);
                 }
 #pragma unroll
-                for (int j = 0; j < GB; j++) s[u * GB + j] = sum[j].x + sum[j].y;
+                for (int j = 0; j < G2; j++) s[u * G2 + j] = j < GB ? sum[j < GB ? j : 0].x + sum[j < GB ? j : 0].y : 0.f;
             }
             issue_v();
             const unsigned now = there >> (RING - 1) / 2 * 4;            // (as many steps are ahead of this one)
@@ -806,12 +810,14 @@ __device__ __forceinline__ bool paged_attention_body(const KTask& t, int vb, uns
 constexpr int kSmsPlanned = 148;                           // launch geometry is planned without a GPU
 // Tensor cores from three query heads to a 16-bit key head on.
 __host__ inline int paged_heads_of_a_pass(int kt, int d, int group) {
-    return group <= 2 ? group : group <= 4 || (kt == KT_FP32 && d == 256) ? 4 : 8;
+    if (kt != KT_FP32) return group <= 2 ? group : group <= 4 ? 4 : 8;
+    const int most = d == 256 ? 4 : 8, passes = (group + most - 1) / most, gb = (group + passes - 1) / passes;
+    return gb == 7 ? 8 : gb;
 }
 __host__ inline bool paged_mma(const PagedP& p) { return p.kt != KT_FP32 && p.gb > 2; }
 struct PagedSimtShape { int unit, scratch; };
 __host__ inline PagedSimtShape paged_simt_shape(const PagedP& p) {      // UNIT and SCRATCH of PagedSimt
-    const int vec = p.kt == KT_FP32 ? 4 : 8, lanes = p.d / vec > 32 ? 32 : p.d / vec, pieces = p.d / (vec * lanes), keys = paged_simt_keys(pieces, p.gb);
+    const int vec = p.kt == KT_FP32 ? 4 : 8, lanes = p.d / vec > 32 ? 32 : p.d / vec, pieces = p.d / (vec * lanes), keys = paged_simt_keys(pieces, lanes, p.gb);
     const int ring = kPagedSimtRing * keys * pieces * 512, slot = p.gb * paged_stride(p.d) * 4;
     return {32 / lanes * keys, ring > slot ? ring : slot};
 }

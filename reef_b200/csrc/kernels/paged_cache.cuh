@@ -383,16 +383,15 @@ __device__ __forceinline__ void append_tokens(const PagedP& p, const KTask& t, i
     const int4* tok = (const int4*)t.a[2];
     C* kc = (C*)t.a[3 + p.has_fork];
     C* vc = (C*)t.a[4 + p.has_fork];
-    const int row = p.kvh * p.d, row4 = row >> 2;
-    const long long total = (long long)p.tokens * row4;
+    const int row4 = p.kvh * p.d >> 2, total = p.tokens * row4, shift = 31 - __clz(p.d);     // (below 2^31: the plan sees to it)
     float4 a[4], b[4];
     C *ka[4], *va[4];
 #pragma unroll
     for (int it = 0; it < 4; it++) {
-        const long long i = (long long)vb * (kAppendPerBlock / 4) + it * kThreads + threadIdx.x;
+        const int i = vb * (kAppendPerBlock / 4) + it * kThreads + threadIdx.x;
         ka[it] = nullptr;
         if (i >= total) continue;
-        const int token = (int)(i / row4), c = (int)(i - (long long)token * row4) << 2, h = c / p.d, e = c - h * p.d;
+        const int token = (int)((unsigned)i / (unsigned)row4), c = (i - token * row4) << 2, h = c >> shift, e = c & (p.d - 1);
         const int slot = tok[token].x;
         if (slot < 0 || slot >= p.pages * p.ps) continue;
         const int page = page_of(p, slot);

@@ -155,7 +155,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
             !maybe_between(a, "ko", 0, 0x7fffffff, 0, &p.qo) || !maybe_between(a, "vo", 0, 0x7fffffff, 0, &p.vo))
             return false;
         if ((p.qs | p.vs | p.qo | p.vo) & 3 || (p.tokens > 1 && (p.qs < row || p.vs < row))) return false;
-        if ((long long)p.rows * p.kvh > (1 << 30)) return false;
+        if ((long long)p.rows * p.kvh > (1 << 30) || (long long)p.tokens * row > 0x70000000LL) return false;
         p.split = append_token_blocks(p);
         t.family = F_PAGED_APPEND;
         t.nblocks = p.split + append_fork_blocks(p);

@@ -271,7 +271,7 @@ TYPES = [F, torch.bfloat16, torch.float16]
 
 @pytest.mark.parametrize("type", TYPES)
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("H,kv", [(1, 1), (4, 2), (6, 2), (12, 12), (5, 1), (14, 2), (8, 1), (16, 1), (24, 1), (40, 2)])
+@pytest.mark.parametrize("H,kv", [(1, 1), (4, 2), (6, 2), (12, 12), (5, 1), (14, 2), (8, 1), (16, 1), (24, 1), (40, 2), (4, 1), (12, 2), (9, 1)])
 @pytest.mark.parametrize("M,S,lens", [(4, 16, [1, 0, 64, 17, 33]), (60, 16, [959, 1, 960, 0, 300]), (700, 3, [2100, 5, 1999])])
 def test_attention(type, D, H, kv, M, S, lens):
     check_attention(*attend_inputs(np.random.default_rng([D, H, M]), lens, H, kv, D, S, M, type))
