@@ -692,48 +692,73 @@ __device__ __forceinline__ bool paged_attention_body(const KTask& t, int vb, uns
             }
         }
     } else {
-        // units of the tokens, a run of tokens to a thread (fewer than 2^31 in all: the plan sees to it)
-        const int per = (p.tokens + kThreads - 1) / kThreads, t0 = min(p.tokens, tid * per), t1 = min(p.tokens, t0 + per);
-        int mine = 0;
-        for (int i = t0; i < t1; i++) mine += (paged_length(p, tok[i]) + E::UNIT - 1) / E::UNIT;
-        int upto = mine;
+        // units of the tokens before each (fewer than 2^31 in all: the plan sees to it); up to 32 tokens every warp counts for itself
+        auto units_of = [&](int i) { return (paged_length(p, tok[i]) + E::UNIT - 1) / E::UNIT; };
+        auto scan = [&](int v) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += u;
-        }
-        if (lane == 31) sl.sums[warp] = upto;
-        __syncthreads();
-        int all = 0, before = 0;
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            if (w < warp) before += sl.sums[w];
-            all += sl.sums[w];
-        }
-        upto += before;
-        const int W = all * P, blocks = min(t.nblocks, (W + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits));
-        // block vb's units and within them warp w's
-        const int each = blocks > 0 ? W / blocks : 0, more = W - each * blocks;
-        const int lo = vb < blocks ? vb * each + min(vb, more) : 0, len = vb < blocks ? each + (vb < more ? 1 : 0) : 0;
-        auto begin_of = [&](int w) { return lo + (int)((unsigned)len * w >> 3); };
-        if (mine > 0 && (upto - mine) * P < lo + len && upto * P > lo)
-            for (int w = 0; w < 8; w++) {
-                const int at = begin_of(w);
-                if (at < (upto - mine) * P || at >= upto * P) continue;
-                int b = upto - mine, i = t0;
-                for (; i < t1; i++) {
-                    const int n = (paged_length(p, tok[i]) + E::UNIT - 1) / E::UNIT;
-                    if (at < (b + n) * P) break;
-                    b += n;
-                }
-                sl.token[w] = i;
-                sl.before[w] = b;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
             }
-        __syncthreads();
-        int u = begin_of(warp);
-        const int end = begin_of(warp + 1);
+            return v;
+        };
+        int all = 0, upto, mine = 0, u, end, token = 0, base = 0;
+        // block vb's units of all, and within them warp w's
+        int lo = 0, len = 0;
+        auto divide = [&]() {
+            const int W = all * P, blocks = min(t.nblocks, (W + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits));
+            const int each = blocks > 0 ? W / blocks : 0, more = W - each * blocks;
+            lo = vb < blocks ? vb * each + min(vb, more) : 0;
+            len = vb < blocks ? each + (vb < more ? 1 : 0) : 0;
+        };
+        auto begin_of = [&](int w) { return lo + (int)((unsigned)len * w >> 3); };
+        if (p.tokens <= 32) {
+            mine = lane < p.tokens ? units_of(lane) : 0;
+            upto = scan(mine);
+            all = __shfl_sync(0xffffffffu, upto, 31);
+            divide();
+            u = begin_of(warp);
+            end = begin_of(warp + 1);
+            token = __popc(__ballot_sync(0xffffffffu, upto * P <= u));
+            base = __shfl_sync(0xffffffffu, (upto - mine) * P, token & 31);
+            __syncthreads();             // (the slots are empty)
+        } else {
+            // a run of tokens to a thread
+            const int per = (p.tokens + kThreads - 1) / kThreads, t0 = min(p.tokens, tid * per), t1 = min(p.tokens, t0 + per);
+            for (int i = t0; i < t1; i++) mine += units_of(i);
+            upto = scan(mine);
+            if (lane == 31) sl.sums[warp] = upto;
+            __syncthreads();
+            int before = 0;
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                if (w < warp) before += sl.sums[w];
+                all += sl.sums[w];
+            }
+            upto += before;
+            divide();
+            if (mine > 0 && (upto - mine) * P < lo + len && upto * P > lo)
+                for (int w = 0; w < 8; w++) {
+                    const int at = begin_of(w);
+                    if (at < (upto - mine) * P || at >= upto * P) continue;
+                    int b = upto - mine, i = t0;
+                    for (; i < t1; i++) {
+                        const int n = units_of(i);
+                        if (at < (b + n) * P) break;
+                        b += n;
+                    }
+                    sl.token[w] = i;
+                    sl.before[w] = b;
+                }
+            __syncthreads();
+            u = begin_of(warp);
+            end = begin_of(warp + 1);
+            if (u < end) {
+                token = sl.token[warp];
+                base = sl.before[warp] * P;
+            }
+        }
         if (u < end) {
-            int token = sl.token[warp], base = sl.before[warp] * P;      // units before this token
             while (u < end && token < p.tokens) {
                 const int4 tk = tok[token];
                 const int n = (paged_length(p, tk) + E::UNIT - 1) / E::UNIT;

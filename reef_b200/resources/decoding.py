@@ -26,10 +26,14 @@ def paged_attention(tokens: int, rows: int, heads: int, kv_heads: int, dim: int,
     (args: parts, out) joins what the first (args: q, k_cache, v_cache, table, tok, out, parts) leaves in ``parts``.
     ``strides``: qs (floats from token to token), qo (floats to the first).
 
-    One kernel while a block reads the longest row's keys and values of a head within about the time of a second launch: 512 KB (12 heads
-    of 64, fp32, a row of 1000: 16.6 us in one kernel, 14.9 and 4.2 in two)."""
+    One kernel leaves a row's keys to one block per key head: no join, and blocks that wait for a free SM even out what SMs and rows differ by;
+    two divide all keys evenly.  Measured (us, one kernel / two, floor; rows of random length up to the longest, whose keys and values of
+    a head are B bytes): 12 heads of one row, B = 512 KB 14.4 / 13.4 for the longest and 6.3 / 12.5 for a short one; 64, 1 MB 27 / 18 (6); 192,
+    512 KB 14.4 / 18, 1 MB 21 / 19 (12); 512, 1 MB 65 / 70 (42); 2048, 2 MB 353 / 383 (343); but 512 of very uneven rows, 4 MB, would wait for
+    the longest.  One kernel, therefore, up to 512 KB and as much again for every 320 heads."""
     shape = dict(tokens=tokens, rows=rows, heads=heads, kvh=kv_heads, d=dim, ps=page_size, mp=max_pages, pages=pages, kt=CACHE_TYPES[cache])
-    if 2 * max_pages * page_size * dim * (4 if cache == "float32" else 2) <= 512 << 10:
+    longest = 2 * max_pages * page_size * dim * (4 if cache == "float32" else 2)
+    if longest <= (512 << 10) * (1 + tokens * kv_heads / 320):
         return [kname("reef_paged_attention", **shape, **strides)]
     return [kname("reef_paged_attention_parts", **shape, **strides), kname("reef_paged_attention_join", **shape)]
 
