@@ -2,6 +2,11 @@
 //   out[t][h] = sum_j p_j v_j,  p = softmax_j(q[t][h] . k_j / sqrt(d)),  j < length of token t,
 // the keys of positions whose page id lies outside the cache left out; zeros where nothing is left.  (The reference attends within
 // a sequence only, resource/bert/bert.cu:22-157.)
+//
+// One pass over the keys with a running maximum and sum; every key and value is read once for up to eight query heads.  Bound by HBM where
+// there is much to read: 64 rows of 32 heads over 8, bf16, 128 dimensions, 860 MB in 157 us (5.5 TB/s, 0.85 of the measured copy rate; SMs
+// do not get equal shares of it), 2048 passes of up to 2 MB 353 us (0.97); fp32 in groups of five, 188 MB in 41 us (0.70).  A
+// call with little to read is a chain of latencies: 12 heads of a row of 77 keys 5.1 us, of 1000 14.
 #pragma once
 #include "bf16_split.cuh"
 #include "paged_cache.cuh"
@@ -133,8 +138,7 @@ struct PagedSimt {
         const bool one_page = r.ps % UNIT == 0;
         int at[U], id[U], pos_in = r.begin;
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (u == 0 || !one_page) id[u] = r.page(r.begin + u * TPI + sub);
+        for (int u = 0; u < U; u++) at[u] = -1, id[u] = r.page(r.begin + u * TPI + sub);
         unsigned there = 0;             // a bit per key of a lane, four to a step, the newest lowest
         auto issue_k = [&]() {
             const uint32_t to = ring.put();
@@ -323,14 +327,15 @@ struct PagedSimt {
 };
 
 // ---- tensor cores -----------------------------------------------------------------------------------------------------------
-// From three query heads to a key head on, the multiplications of the fp32 form are what takes the time; 16-bit keys and values are
-// operands of mma.sync as they are.  Queries and probabilities keep their 32 bits: a query is the sum of three bf16 values (or two fp16
-// values, scaled to the type's range), exactly, and of the sixteen rows of a multiplication eight heads take up two: the products of the first
-// part in rows 0 - 7, of the second in rows 8 - 15 of the same instruction, where one lane holds both.  Sums are carried on outside the
-// tensor core, whose additions truncate.
-// A warp takes 16 keys at a time, straight from global memory into registers in the operands' layout: lane (g, c) has 16-byte pieces of
-// keys g and 8 + g, whose eight dimensions are its K positions of two instructions; and of the values of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-// eight dimensions, which are its columns of eight instructions.
+// From three query heads to a key head on, the multiplications of the fp32 form are what takes the time (64 rows of 32 heads over 8 as above:
+// 375 us); 16-bit keys and values are operands of mma.sync as they are.  Queries and probabilities keep their 32 bits: a bf16 query is the
+// exact sum of three bf16 values, an fp16 one that of two fp16 values, scaled to the type's range, but for 2^-22 of it.  The sixteen rows of
+// a multiplication hold four or eight heads' parts side by side, so that one instruction, or two, multiplies all of them.  Sums are carried on
+// outside the tensor core, whose additions truncate.
+// A warp takes 16 keys at a time, from its ring into registers in the operands' layout: lane (g, c) has 16-byte pieces of keys g and 8 + g,
+// whose eight dimensions are its K positions of two instructions; and of the values of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 eight dimensions,
+// which are its columns of eight instructions.  These multiplications keep the tensor pipe 28 % busy while HBM is the bound, so that the
+// 128 rows of a tcgen05 tile would wait for the same bytes.
 // What the parts cannot carry (an infinity or NaN among the operands) ends as a sum that is not finite: such a range is worked out again by
 // fp32 instructions.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
