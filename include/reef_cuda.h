@@ -155,7 +155,8 @@ typedef struct {
     int max_blocks_per_sm; /* occupancy from the CUDA occupancy API at (threads, dyn_smem)  */
     double flops;          /* algorithmic FLOPs of one launch                               */
     double bytes;          /* algorithmic HBM bytes of one launch                           */
-    int tensor_core;       /* 1 when the kernel's contraction runs on tcgen05               */
+    int tensor_core;       /* 1 when the kernel's contraction runs on tcgen05, or it is otherwise a kernel of
+                              its own that the dispatcher does not host (a block to half an SM) */
     int cluster;           /* thread blocks per cluster (1 = no cluster); block ranges handed to
                               reef_dispatch for this kernel must be multiples of it           */
     int chainable;         /* 1: a tensor-core convolution / matmul that reef_chain_create accepts */
@@ -216,8 +217,8 @@ REEF_API reef_status reef_dispatch(reef_kernel_t rt, void** rt_args,
  *    tickets.  Give concurrent streams different lanes.
  *  - The first call on a device looks up the array's device address (cudaGetSymbolAddress, with that device
  *    current); make that first call before any stream capture begins.
- *  - Logical-block kernels only (one persistent grid); a tensor-core cluster kernel on either side is
- *    refused with REEF_FAIL.  Everything else is as in reef_dispatch's single-grid form. */
+ *  - Logical-block kernels only (one persistent grid); a tensor-core cluster kernel, or another one that is
+ *    launched on its own (attrs.tensor_core), on either side is refused with REEF_FAIL.  Everything else is as in reef_dispatch's single-grid form. */
 #define REEF_STATIC_DISPATCH_LANES 64
 REEF_API reef_status reef_dispatch_static(reef_kernel_t rt, void** rt_args,
                                           reef_kernel_t be, void** be_args,

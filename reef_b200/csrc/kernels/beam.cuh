@@ -13,8 +13,8 @@ constexpr int kBeamMax = 16;
 constexpr int kBeamVecs = 4;                              // 128-bit loads of a lane and turn
 constexpr int kBeamTurn = kBeamVecs * 4 * 32;             // words of a warp's turn
 constexpr int kBeamRoom = 512;                            // candidates that a block ranks side by side
-// Parts of a row of logits, a part to a block: a turn of its eight warps at least, and over all rows not more blocks than four to an SM
-// or, from there on, whole rounds of as many.
+// Parts of a row of logits, a part to a block: a turn of its eight warps at least, and over all rows not more than four blocks to an SM
+// (a second round of blocks repeats what a block has to do once: 256 rows in 2 parts each 39 us, in 4 parts 50, in 1 part 41).
 __host__ inline int beam_parts(long long rows, int vocab) {
     const long long least = 8LL * kBeamTurn, most = (vocab + least - 1) / least, slots = 4 * 148;
     if (rows * most <= slots) return (int)most;
@@ -120,8 +120,7 @@ __device__ __forceinline__ int beam_logits(const BeamP& p, const int* start, int
 // maximum and a sum of its own, the next turn's loads are under way while a turn is looked at.  The greatest words so far stand in their
 // order in the warp's first K lanes; a word that is greater than the last of them moves in by a shuffle.  What keeps that rare: the first
 // turn begins with the K-th greatest of the lanes' maxima as a line, and the greatest line of the block's warps holds for all of them.
-// HBM, or L2 where the projection has just left the logits, would bound it; what does are the instructions of words that move in (all of
-// them taken out: 30 us): 256 rows of 100003 words, 95 MB, 39 us (0.37 of the measured copy rate), 61 with a room in shared memory that was
+// HBM, or L2 where the projection has just left the logits, would bound it; what does are instructions: 256 rows of 100003 words, 95 MB, 39 us (0.37 of the measured copy rate), 61 with a room in shared memory that was
 // ranked whenever it filled; four rows of 30522 words 8.
 struct BeamScan {
     float value[8][kBeamMax];
@@ -303,7 +302,7 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
 // ---- pick: the parts of a request's beams -> its new beams --------------------------------------------------------------------
 // args: parts, score, live, [start], token, parent, score', live'.  Within a beam the logits decide, exactly as they are; beams are
 // compared in 64 bits: a score of -50 in 32 bits cannot tell logits apart that differ by less than 4e-6.  Latency: 32 requests of eight beams
-// 8 us, of them 3 for the logarithm and exponentials in 64 bits.
+// 8 us.
 __host__ inline int beam_pick_smem() { return kBeamSmem + kBeamMax * (8 + 8 + 4 + 4); }
 __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned char* smem, const int*) {
     const BeamP& p = t.p.beam;

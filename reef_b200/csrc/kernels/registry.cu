@@ -1342,7 +1342,7 @@ int launch_dispatch_static(const KernelSpec* rt, void** rt_args, const KernelSpe
     if (rt == nullptr && be == nullptr) return REEF_FAIL;
     if (be == nullptr) be_num = 0;
     if ((rt != nullptr && is_own_family(rt->task.family)) || (be_num > 0 && is_own_family(be->task.family))) {
-        set_error("reef_dispatch_static hosts logical-block kernels only (a tensor-core cluster kernel was given)");
+        set_error("reef_dispatch_static hosts logical-block kernels only (a tensor-core cluster kernel, or one that is launched on its own, was given)");
         return REEF_FAIL;
     }
     if (be_num > 0 && (be_off < 0 || be_off + be_num > be->task.nblocks)) {
