@@ -386,29 +386,28 @@ __device__ __forceinline__ void append_tokens(const PagedP& p, const KTask& t, i
     C* kc = (C*)t.a[3 + p.has_fork];
     C* vc = (C*)t.a[4 + p.has_fork];
     const int row4 = p.kvh * p.d >> 2, total = p.tokens * row4, shift = 31 - __clz(p.d);     // (below 2^31: the plan sees to it)
+    // the loads do not wait for the slots
     float4 a[4], b[4];
-    C *ka[4], *va[4];
+    int token[4], c[4];
 #pragma unroll
     for (int it = 0; it < 4; it++) {
         const int i = vb * (kAppendPerBlock / 4) + it * kThreads + threadIdx.x;
-        ka[it] = nullptr;
+        token[it] = -1;
         if (i >= total) continue;
-        const int token = (int)((unsigned)i / (unsigned)row4), c = (i - token * row4) << 2, h = c >> shift, e = c & (p.d - 1);
-        const int slot = tok[token].x;
-        if (slot < 0 || slot >= p.pages * p.ps) continue;
-        const int page = page_of(p, slot);
-        const size_t at = (((size_t)page * p.kvh + h) * p.ps + (slot - page * p.ps)) * p.d + e;
-        ka[it] = kc + at;
-        va[it] = vc + at;
-        a[it] = *reinterpret_cast<const float4*>(k + (size_t)token * p.qs + c);
-        b[it] = *reinterpret_cast<const float4*>(v + (size_t)token * p.vs + c);
+        token[it] = (int)((unsigned)i / (unsigned)row4);
+        c[it] = (i - token[it] * row4) << 2;
+        a[it] = *reinterpret_cast<const float4*>(k + (size_t)token[it] * p.qs + c[it]);
+        b[it] = *reinterpret_cast<const float4*>(v + (size_t)token[it] * p.vs + c[it]);
     }
 #pragma unroll
-    for (int it = 0; it < 4; it++)
-        if (ka[it]) {
-            store4(ka[it], a[it]);
-            store4(va[it], b[it]);
-        }
+    for (int it = 0; it < 4; it++) {
+        const int slot = token[it] >= 0 ? tok[token[it]].x : -1;
+        if (slot < 0 || slot >= p.pages * p.ps) continue;
+        const int page = page_of(p, slot), h = c[it] >> shift, e = c[it] & (p.d - 1);
+        const size_t at = (((size_t)page * p.kvh + h) * p.ps + (slot - page * p.ps)) * p.d + e;
+        store4(kc + at, a[it]);
+        store4(vc + at, b[it]);
+    }
 }
 
 __device__ __forceinline__ bool body_paged_append(const KTask& t, int vb, unsigned char*, const int*) {
