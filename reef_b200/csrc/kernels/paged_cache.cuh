@@ -48,50 +48,57 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // Used pages are marked in bytes, a window of the pages at a time, and packed to bits: an atomic OR into a word of bits took 1.5 cycles for
 // every id, 53 us for 62500 of them, a byte is a plain store.  A free page is found by its rank (a prefix sum over the threads' words, a walk
 // through one thread's), by whoever needs it.  16 rows of 500 tokens 7 us, 128 beams 12, 256 rows of two million tokens in all (62500 ids)
-// 28 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them).
+// 23 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them).
+constexpr int kTablesThreads = 2 * kThreads;
 constexpr int kTablesMaxRows = 1024, kTablesMaxPages = 1 << 19;
-__host__ __device__ constexpr int tables_fixed(int rows, int pages) { return (4 * ((pages + 31) / 32 + 8 * rows + 3 + 24 + 260) + 15) / 16 * 16; }
+__host__ __device__ constexpr int tables_fixed(int rows, int pages) { return (4 * ((pages + 31) / 32 + 8 * rows + 2 + 96 + kTablesThreads) + 15) / 16 * 16; }
 __host__ __device__ constexpr int tables_window(int rows, int pages) {      // what fits an SM beside the rest
     const int all = (pages + 31) / 32 * 32, room = (225 * 1024 - tables_fixed(rows, pages)) / 512 * 512;
     return all < room ? all : room;
 }
 __host__ constexpr int tables_smem(int rows, int pages) { return tables_fixed(rows, pages) + tables_window(rows, pages); }
 constexpr int kTablesSmemMax = 225 * 1024;
+// Twice the threads from 8192 ids on: 64 rows of 512 ids 12.4 us instead of 14.4, 256 rows of 1024 22.7 instead of 26.8, 16 rows of 64
+// 11.2 instead of 10.4.  1024 threads do less, their barriers and sums cost more than they divide: 16.5, 24.3 and 12.4.  A dispatcher's
+// blocks, which have kThreads, do the same work.
+__host__ inline int tables_threads(int rows, int max_pages) { return (long long)rows * max_pages >= 8192 ? kTablesThreads : kThreads; }
 // Rows and tokens are written by up to 32 blocks, 4096 ids or 256 tokens to a block.
 __host__ inline int tables_blocks(int rows, int max_pages, int tokens) {
     const long long want = max(((long long)rows * max_pages + 4095) / 4096, (long long)(tokens + 255) / 256);
     return (int)min(want, 32LL);
 }
 
-// inclusive sums over 256 threads in their order, of N values side by side; returns the exclusive ones in v, the totals in all
+// sums over a block's threads in their order, of N values side by side; returns the exclusive ones in v, the totals in all
 template <int N>
 __device__ __forceinline__ void block_scan(int (&v)[N], int (&all)[N], int* sums) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x[N];
-#pragma unroll
-    for (int n = 0; n < N; n++) {
-        x[n] = v[n];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int x[N], y[N];
+    auto scan = [&](int (&z)[N]) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, x[n], o);
-            if (lane >= o) x[n] += u;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const int u = __shfl_up_sync(0xffffffffu, z[n], o);
+                if (lane >= o) z[n] += u;
+            }
         }
-    }
+    };
+#pragma unroll
+    for (int n = 0; n < N; n++) x[n] = v[n];
+    scan(x);
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < N; n++)
-        if (lane == 31) sums[8 * n + warp] = x[n];
+        if (lane == 31) sums[32 * n + warp] = x[n];
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-        int before = 0;
-        all[n] = 0;
+    for (int n = 0; n < N; n++) y[n] = lane < warps ? sums[32 * n + lane] : 0;
+    scan(y);
 #pragma unroll
-        for (int w = 0; w < 8; w++) {
-            if (w < warp) before += sums[8 * n + w];
-            all[n] += sums[8 * n + w];
-        }
-        v[n] = x[n] - v[n] + before;
+    for (int n = 0; n < N; n++) {
+        const int before = __shfl_sync(0xffffffffu, y[n], max(warp - 1, 0));
+        all[n] = __shfl_sync(0xffffffffu, y[n], 31);
+        v[n] = x[n] - v[n] + (warp ? before : 0);
     }
 }
 // the last i in [lo, hi) with a[i] <= x (a does not fall, a[lo] <= x)
@@ -116,11 +123,11 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
     int4* tok_out = (int4*)t.a[6 + f];
     int* status_out = (int*)t.a[7 + f];
     int4* fork_out = f ? (int4*)t.a[9] : nullptr;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = (N + 31) / 32;
+    const int threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = (N + 31) / 32;
     unsigned* open = (unsigned*)smem;              // a bit per page: used, later free
     int* sums = (int*)(open + words);              // scratch of the prefix sums
-    int* holes = sums + 24;                        // free pages before every thread's words [256 + 1]
-    int* len = holes + 260;                        // per row: tokens held
+    int* holes = sums + 96;                        // free pages before every thread's words
+    int* len = holes + kTablesThreads;                      // per row: tokens held
     int* add = len + R;                            // tokens added
     int* from = add + R;                           // row it goes on from, -1 for none
     int* state = from + R;                         // status; -1 accepted with a copy of the last page
@@ -132,7 +139,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
     const int window = tables_window(R, N);
     const bool wide = (M & 3) == 0 && ((uintptr_t)table & 15) == 0;         // rows begin at 16-byte boundaries
     __syncthreads();                               // a persistent caller's previous block is out of shared memory
-    for (int r = tid; r < R; r += kThreads) {
+    for (int r = tid; r < R; r += threads) {
         const int q = f ? parent[r] : r;
         const bool named = q >= -1 && q < R;
         const int l = named && q >= 0 ? lens[q] : 0, n = fresh[r];
@@ -144,16 +151,16 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
     }
     __syncthreads();
     if (f) {
-        for (int r = tid; r < R; r += kThreads)
+        for (int r = tid; r < R; r += threads)
             if (from[r] >= 0) atomicMin(&owner[from[r]], r);
         __syncthreads();
     }
-    // a thread's rows, at most four, in their order
-    const int per = (R + kThreads - 1) / kThreads, r0 = tid * per, r1 = min(R, r0 + per);
+    // a thread's rows in their order
+    const int per = (R + threads - 1) / threads, r0 = tid * per, r1 = min(R, r0 + per);
     auto kept = [&](int r) { return page_of(p, len[r] + S - 1); };
     auto pieces = [&](int r) { return state[r] == 0 && from[r] >= 0 && owner[from[r]] == r ? (kept(r) + 127) >> 7 : 0; };
     // bits of the pages that no row keeps; `part` of them among this thread's words
-    const int wper = (words + kThreads - 1) / kThreads, w0 = min(words, tid * wper), w1 = min(words, w0 + wper);
+    const int wper = (words + threads - 1) / threads, w0 = min(words, tid * wper), w1 = min(words, w0 + wper);
     int part[3] = {0, 0, 0}, all[3];
     for (int pass = 0; pass < 2; pass++) {         // (a second time without the rows whose ids are out of range, if there are any)
         int count1[1] = {0}, all1[1];
@@ -166,11 +173,11 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
         if (tid == 0) base[R] = all1[0];
         bool wrong = false;
         for (int first = 0; first < N; first += window) {
-            for (int i = tid * 16; i < window; i += kThreads * 16) *reinterpret_cast<uint4*>(mark + i) = make_uint4(0, 0, 0, 0);
+            for (int i = tid * 16; i < window; i += threads * 16) *reinterpret_cast<uint4*>(mark + i) = make_uint4(0, 0, 0, 0);
             __syncthreads();
-            for (int c0 = 0; c0 < all1[0]; c0 += kThreads) {
-                // every eighth piece to a warp, 32 of them at a time: a lane looks up the row of one
-                const int c = c0 + warp + 8 * lane;
+            for (int c0 = 0; c0 < all1[0]; c0 += threads) {
+                // the pieces go round the warps, 32 of them at a time: a lane looks up the row of one
+                const int c = c0 + warp + warps * lane;
                 int at = 0, left = 0, row = 0;
                 if (c < all1[0]) {
                     row = last_below(base, 0, R, c);
@@ -179,7 +186,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                     at = from[row] * M + j;                                             // (rows * max_pages is at most 2^30)
                     if (left <= 128 && len[row] != kept(row) * S) left |= 1 << 30;     // its last id names a page that is written
                 }
-                const int n = min(32, (all1[0] - c0 - warp + 7) >> 3);
+                const int n = min(32, (all1[0] - c0 - warp + warps - 1) / warps);
 #pragma unroll 1
                 for (int i0 = 0; i0 < n; i0 += 8) {
                     int4 id[8];
@@ -223,7 +230,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                 }
             }
             __syncthreads();
-            for (int w = tid; w < window / 32 && first / 32 + w < words; w += kThreads) {
+            for (int w = tid; w < window / 32 && first / 32 + w < words; w += threads) {
                 const uint4* b = reinterpret_cast<const uint4*>(mark + w * 32);
                 unsigned x = 0;
 #pragma unroll
@@ -238,7 +245,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
             }
         }
         if (!__syncthreads_or(wrong)) break;
-        for (int r = tid; r < R; r += kThreads)
+        for (int r = tid; r < R; r += threads)
             if (from[r] >= 0 && bad[from[r]]) state[r] = 2;
         __syncthreads();
     }
@@ -295,7 +302,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
     __syncthreads();
     // the free page of a rank
     auto free_page = [&](int rank) {
-        const int th = last_below(holes, 0, kThreads, rank);
+        const int th = last_below(holes, 0, threads, rank);
         int w = th * wper, left = rank - holes[th], n = __popc(open[w]);
         while (left >= n) {
             left -= n;
@@ -311,7 +318,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
         return j < copied ? table[(size_t)from[r] * M + j] : free_page(base[r] + j - copied);
     };
     const int rows_per = (R + p.split - 1) / p.split, mine0 = min(R, vb * rows_per), mine1 = min(R, mine0 + rows_per);
-    for (int r = mine0 + warp; r < mine1; r += 8) {
+    for (int r = mine0 + warp; r < mine1; r += warps) {
         const int total = page_of(p, len[r] + add[r] + S - 1), copied = kept(r) - (state[r] < 0 ? 1 : 0);
         const int* ids = table + (size_t)max(from[r], 0) * M;
         int* to = table_out + (size_t)r * M;
@@ -331,7 +338,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
         }
         for (int j = copied + lane; j < total; j += 32) to[j] = free_page(base[r] + j - copied);
     }
-    for (int r = mine0 + tid; r < mine1; r += kThreads) {
+    for (int r = mine0 + tid; r < mine1; r += threads) {
         lens_out[r] = len[r] + add[r];
         start_out[r] = begin[r];
         status_out[r] = max(state[r], 0);
@@ -341,7 +348,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
         }
     }
     if (vb == 0 && tid == 0) start_out[R] = begin[R];
-    for (int i = vb * kThreads + tid; i < p.tokens; i += p.split * kThreads) {
+    for (int i = vb * threads + tid; i < p.tokens; i += p.split * threads) {
         int4 x = make_int4(-1, -1, 0, 0);
         if (i < begin[R]) {
             const int r = last_below(begin, 0, R, i), pos = len[r] + i - begin[r], j = page_of(p, pos);
@@ -357,7 +364,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
 // (to nearest even: the type is the caller's choice); tokens without a slot are passed over.  A fork (src, dst, n) copies the
 // first n tokens of a page; new tokens are written behind them, and src's first n are written by nobody, so the order of the
 // two does not matter and a second run gives the same.  Bound by HBM: every byte is moved once, 16 at a time, eight loads of a thread under
-// way: 8192 tokens of 8 heads of 128 into bf16, 100 MB, 21.8 us (0.72 of the measured copy rate), 128 beams with 40 forks 4.1.
+// way: 8192 tokens of 8 heads of 128 into bf16, 100 MB, 21.0 us (0.74 of the measured copy rate), 128 beams with 40 forks 4.1.
 constexpr int kAppendPerBlock = 4 * kThreads * 4;       // fp32 values of k, and of v
 __host__ inline int append_token_blocks(const PagedP& p) {
     return (int)(((long long)p.tokens * p.kvh * p.d + kAppendPerBlock - 1) / kAppendPerBlock);

@@ -140,6 +140,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
         p.split = tables_blocks(p.rows, p.mp, p.tokens);
         t.family = F_PAGE_TABLES;
         t.nblocks = p.split;
+        s->block[0] = (uint32_t)tables_threads(p.rows, p.mp);
         s->dyn_smem = (uint32_t)tables_smem(p.rows, p.pages);
         s->nargs = p.has_fork ? 10 : 8;
         s->bytes = 4.0 * (2.0 * p.rows * p.mp + 4.0 * p.tokens + (p.has_fork ? 10.0 : 5.0) * p.rows);
@@ -868,8 +869,11 @@ __device__ __forceinline__ void preempt_stamp_leave() {
 // Two blocks per SM where the body's registers would otherwise leave room for one.
 constexpr int min_blocks(int family) { return family == F_CONV_SIMT || family == F_ATTENTION_STAGED ? 2 : family == F_BEAM_SCAN ? 4 : 1; }
 
+// threads of a block launched by itself, at most
+constexpr int max_threads(int family) { return family == F_PAGE_TABLES ? kTablesThreads : kThreads; }
+
 template <int F>
-__global__ void __launch_bounds__(kThreads, min_blocks(F)) k_plain(const __grid_constant__ KTask t) {
+__global__ void __launch_bounds__(max_threads(F), min_blocks(F)) k_plain(const __grid_constant__ KTask t) {
     if (F == F_LAYERNORM) prefetch_layernorm(t);
     if (F == F_DENSE) prefetch_dense(t, blockIdx.x);
     run_body<F>(t, blockIdx.x, reef_dyn_smem, nullptr, EnterPlain());
@@ -879,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, min_blocks(F)) k_plain(const __grid_
 // the preempt flag is up; bodies poll it again at their loop heads; a block that ran to the end
 // (all of its stores issued) adds one to the kernel's completion counter.
 template <int F>
-__global__ void __launch_bounds__(kThreads, min_blocks(F)) k_be(const __grid_constant__ KTask t, const int* __restrict__ flag,
+__global__ void __launch_bounds__(max_threads(F), min_blocks(F)) k_be(const __grid_constant__ KTask t, const int* __restrict__ flag,
                                                  int* __restrict__ task_slot) {
     if (F == F_LAYERNORM) prefetch_layernorm(t);
     if (F == F_DENSE) prefetch_dense(t, blockIdx.x);

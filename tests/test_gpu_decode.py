@@ -106,6 +106,15 @@ def test_page_tables(R, M, S, pages, tokens, forks):
         check_tables(table, lens, new, parent, pages, S, tokens)
 
 
+@pytest.mark.parametrize("pages", [230000, 1 << 19])
+def test_page_tables_of_more_pages_than_a_window_marks(pages):
+    rng = np.random.default_rng(pages)
+    R, M, S = 40, 8200, 2
+    table, lens = random_rows(rng, R, M, S, pages, 10000)
+    for parent in (None, np.arange(R) // 2 * 2):
+        check_tables(table, lens, rng.integers(0, 40, R), parent, pages, S, 900)
+
+
 @pytest.mark.parametrize("bad", ["len", "len_long", "new", "new_long", "id", "id_low", "parent", "parent_low", "last_gone"])
 def test_page_tables_refuse_single_rows(bad):
     rng = np.random.default_rng(3)

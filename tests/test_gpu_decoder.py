@@ -227,6 +227,37 @@ def test_attention_with_parts_is_preempted_and_resumed(tmp_path):
     e.close()
 
 
+@pytest.mark.parametrize("rows,most", [(16, 64), (70, 130)])
+def test_tables_in_every_flavour(tmp_path, rows, most):
+    """The blocks of a launch of its own and those of a dispatcher give the same tables, whatever their threads."""
+    from reef_b200.resources import decoding
+    from reef_b200.resources.graph import Graph
+    size, pages, tokens = 4, 12000, 200
+    g = Graph("tables")
+    rng = np.random.default_rng(rows)
+    lens, new, parent = rng.integers(0, most * size - 4, rows), rng.integers(0, 4, rows), np.arange(rows) // 2 * 2
+    table, ids, at = np.full((rows, most), -1), rng.permutation(pages), 0
+    for r in range(rows):
+        n = -(-int(lens[r]) // size)
+        table[r, :n] = ids[at:at + n]
+        at += n
+    names = ("table", "lens", "new", "parent", "table_out", "lens_out", "start", "tok", "status", "fork")
+    name = decoding.page_tables(rows, most, size, pages, tokens, fork=True)
+    k = capi.Kernel(name)
+    sizes = [k.arg_bytes[i] // 4 for i in range(10)]
+    bufs = [g.input(n, sizes[i], "int32") if i < 4 else g.add_storage("output" if n == "table_out" else n, sizes[i], "int32") for i, n in enumerate(names)]
+    g.kernel(name, bufs)
+    e = load_executor(g.write(str(tmp_path), capi.plan_fn), params=False)
+    for n, v in zip(names, (table, lens, new, parent)):
+        e.set_input(n, v.astype(np.int32))
+    want = tables_by_hand(table, lens, new, parent, pages, size, tokens)
+    for run in (e.execute, e.execute_graph, e.execute_preemptable, e.execute_dispatch):
+        run()
+        for b, n, y in zip(bufs[4:], sizes[4:], want):
+            assert np.array_equal(e.get_data(b, 4 * n, np.int32), y.ravel())
+    e.close()
+
+
 def test_a_step_on_tensors():
     """The operators one after the other on torch tensors, captured as one graph and replayed, against an uncached computation."""
     torch.manual_seed(0)
