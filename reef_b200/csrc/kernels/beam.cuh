@@ -2,8 +2,7 @@
 //   cand(b, w) = score[b] + logits[b][w] - log sum_u exp(logits[b][u]),
 // ties by the lowest b * vocab + w.  A beam that has ended (live 0) competes with its score and the end word alone; candidates of
 // -infinity or NaN are none, so a row without a finite sum (a NaN, an infinity, nothing but -infinity) has none, nor has a beam without a
-// finite score.  What is missing comes
-// out as token -1, parent -1, score -infinity, live 0.
+// finite score.  What is missing comes out as token -1, parent -1, score -infinity, live 0.
 #pragma once
 #include "paged_cache.cuh"
 
@@ -14,7 +13,7 @@ constexpr int kBeamVecs = 4;                              // 128-bit loads of a 
 constexpr int kBeamTurn = kBeamVecs * 4 * 32;             // words of a warp's turn
 constexpr int kBeamRoom = 512;                            // candidates that a block ranks side by side
 // Parts of a row of logits, a part to a block: a turn of its eight warps at least, and over all rows not more than four blocks to an SM
-// (a second round of blocks repeats what a block has to do once: 256 rows in 2 parts each 39 us, in 4 parts 50, in 1 part 41).
+// (a second round of blocks repeats what a block has to do once: 256 rows in 2 parts each 23 us, in 4 parts 27, in 1 part 31).
 __host__ inline int beam_parts(long long rows, int vocab) {
     const long long least = 8LL * kBeamTurn, most = (vocab + least - 1) / least, slots = 4 * 148;
     if (rows * most <= slots) return (int)most;
@@ -36,10 +35,35 @@ constexpr int kBeamSmem = (int)sizeof(BeamRoom<double>);
 template <class V>
 __device__ __forceinline__ bool beam_before(V a, int ia, V b, int ib) { return a > b || (a == b && ia < ib); }
 
-// The K greatest of all threads' values in their order, ties by the lowest index; `each(f)` calls f(value, index) for those of this
-// thread, -infinity and NaN are none.  Every warp's K-th greatest of its lanes' maxima has K values at or above it, so the greatest of
-// these eight is a line that few values reach: those are ranked against each other.  Where more reach it than there is room (many equal
-// values) the best one behind the last is looked for K times.  `take(i, value, index)` gets the i-th; returns how many there are.
+// `each(f)` calls f(value, index) for the values of this thread; -infinity and NaN are none.  block_collect gathers those of all threads (s.count
+// is 0 before, the threads have not met behind it), block_place ranks them, if there is room for all, ties by the lowest index, and calls
+// `take(i, value, index)` for the i-th of the K greatest; both it and block_top return how many of these there are.
+template <class V, class Each>
+__device__ __forceinline__ void block_collect(BeamRoom<V>& s, Each each) {
+    each([&](V v, int i) {
+        if (v > (V)-INFINITY) {
+            const int at = atomicAdd(&s.count, 1);
+            if (at < kBeamRoom) {
+                s.value[at] = v;
+                s.index[at] = i;
+            }
+        }
+    });
+}
+template <class V, class Take>
+__device__ __forceinline__ int block_place(int K, const BeamRoom<V>& s, int n, Take take) {
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+        const V v = s.value[c];
+        const int i = s.index[c];
+        int r = 0;
+#pragma unroll 4
+        for (int o = 0; o < n; o++) r += beam_before(s.value[o], s.index[o], v, i);
+        if (r < K) take(r, v, i);
+    }
+    return min(n, K);
+}
+// Every warp's K-th greatest of its lanes' maxima has K values at or above it, so the greatest of these eight is a line that few values
+// reach.  Where more reach it than there is room for (many equal values) the best one behind the last is looked for K times.
 template <class V, class Each, class Take>
 __device__ __forceinline__ int block_top(int K, BeamRoom<V>& s, Each each, Take take) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -59,27 +83,10 @@ __device__ __forceinline__ int block_top(int K, BeamRoom<V>& s, Each each, Take 
     V line = s.line[0];
 #pragma unroll
     for (int w = 1; w < 8; w++) line = s.line[w] > line ? s.line[w] : line;
-    each([&](V v, int i) {
-        if (v >= line && v > ninf) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kBeamRoom) {
-                s.value[at] = v;
-                s.index[at] = i;
-            }
-        }
-    });
+    block_collect<V>(s, [&](auto f) { each([&](V v, int i) { if (v >= line) f(v, i); }); });
     __syncthreads();
     const int n = s.count;
-    if (n <= kBeamRoom) {
-        for (int c = tid; c < n; c += kThreads) {
-            const V v = s.value[c];
-            const int i = s.index[c];
-            int r = 0;
-            for (int o = 0; o < n && r < K; o++) r += beam_before(s.value[o], s.index[o], v, i);
-            if (r < K) take(r, v, i);
-        }
-        return min(n, K);
-    }
+    if (n <= kBeamRoom) return block_place<V>(K, s, n, take);
     V last = INFINITY;
     int last_i = -1, found = 0;
     for (; found < K; found++) {
@@ -116,17 +123,20 @@ __device__ __forceinline__ int beam_logits(const BeamP& p, const int* start, int
 }
 
 // ---- scan: a part of a row of logits -> its maximum, the sum of exponentials below it, its `beams` greatest ------------------
-// args: logits, live, [start], parts.  One pass, a range of the part to a warp, no warp waiting for another until the end: a lane carries a
-// maximum and a sum of its own, the next turn's loads are under way while a turn is looked at.  The greatest words so far stand in their
-// order in the warp's first K lanes; a word that is greater than the last of them moves in by a shuffle.  What keeps that rare: the first
-// turn begins with the K-th greatest of the lanes' maxima as a line, and the greatest line of the block's warps holds for all of them.
-// HBM, or L2 where the projection has just left the logits, would bound it; what does are instructions: 256 rows of 100003 words, 95 MB, 39 us (0.37 of the measured copy rate), 61 with a room in shared memory that was
-// ranked whenever it filled; four rows of 30522 words 8.
+// args: logits, live, [start], parts.  One pass, a range of the part to a warp, no warp waiting for another until the end: a lane carries the
+// maximum of its words, the turn that it came in, and a sum below it; the next turn's loads are under way while a turn is looked at.  The lanes
+// are divided into 16 groups, or 32 for more beams than 8, whose words lie all over the part.  K groups have a word at or above the K-th
+// greatest of their maxima, so nothing but what reaches that line (words above it, and those equal to it up to its turn) can be among
+// the K greatest.  The words of the lanes whose maxima reach it, some 12 of 256, are read again, from L2, and those that do are ranked.
+// 256 rows of 100003 words, 102 MB, 23 us (0.70 of the measured copy rate; 39 with the greatest words kept in order as they came, 61 with a room
+// in shared memory that was ranked whenever it filled), of these 19 for the pass and the rest for the line, the second look and the ranking,
+// during which nothing is read; four rows of 30522 words 6.  Code of many unrolled steps after the pass is itself slow, every line of
+// it being fetched once: a loop unrolled 16 times took 1 us longer than the loop.
 struct BeamScan {
-    float value[8][kBeamMax];
-    int index[8][kBeamMax];
+    BeamRoom<float> room;
+    float key[8][32];            // of every warp and group the greatest word and the turn it came in
+    int turn[8][32];
     float top[8], sum[8];
-    float line;                  // K words of the part are at or above it
 };
 __device__ __forceinline__ float2 exp_two(float x, float y, float top) {     // e^(x - top), e^(y - top)
     float2 d = add2(make_float2(x, y), make_float2(-top, -top));
@@ -150,48 +160,23 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
     const int each_warp = loads > 0 ? ((loads + 7) / 8 + 31) / 32 * 32 : 0;
     const int begin = (first + warp * each_warp) * 4 - lead, end = min(p.vocab, (first + min(loads, (warp + 1) * each_warp)) * 4 - lead);
     float4 x[kBeamVecs], next[kBeamVecs];
+    auto load_at = [&](int w, int end) {
+        if (w >= 0 && w + 4 <= end) return *reinterpret_cast<const float4*>(logits + w);
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e] = w + e >= 0 && w + e < end ? logits[w + e] : -INFINITY;
+        return make_float4(z[0], z[1], z[2], z[3]);
+    };
     auto load = [&](float4 (&y)[kBeamVecs], int at) {
 #pragma unroll
-        for (int i = 0; i < kBeamVecs; i++) {
-            const int w = at + (i * 32 + lane) * 4;
-            if (w >= 0 && w + 4 <= end) {
-                y[i] = *reinterpret_cast<const float4*>(logits + w);
-            } else {
-                float z[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) z[e] = w + e >= 0 && w + e < end ? logits[w + e] : -INFINITY;
-                y[i] = make_float4(z[0], z[1], z[2], z[3]);
-            }
-        }
+        for (int i = 0; i < kBeamVecs; i++) y[i] = load_at(at + (i * 32 + lane) * 4, end);
     };
-    int here = begin;                          // first word of this turn
+    int here = begin, turn = 0;                // first word of this turn, and of the one with this lane's maximum
     float top = -INFINITY;
     float2 sum = make_float2(0.f, 0.f);
-    // this lane's word among the K greatest; the last of them
-    float mine = -INFINITY, last = -INFINITY;
-    int mine_i = 0x7fffffff, last_i = 0x7fffffff;
-    auto move_in = [&](float v, int w) {       // (the same v and w in all lanes; it comes before the last)
-        const int at = __popc(__ballot_sync(0xffffffffu, lane < K && beam_before(mine, mine_i, v, w)));
-        const float pv = __shfl_up_sync(0xffffffffu, mine, 1);
-        const int pi = __shfl_up_sync(0xffffffffu, mine_i, 1);
-        if (lane >= at) {
-            mine = lane == at ? v : pv;
-            mine_i = lane == at ? w : pi;
-        }
-        last = __shfl_sync(0xffffffffu, mine, K - 1);
-        last_i = __shfl_sync(0xffffffffu, mine_i, K - 1);
-    };
-    // the greatest line of the block's warps: as an integer a float >= 0 keeps its order, a float < 0 has it turned round
-    auto raise = [&](float v) {
-        if (v >= 0.f) atomicMax((int*)&s.line, __float_as_int(v));
-        else atomicMin((unsigned*)&s.line, __float_as_uint(v));
-    };
     bool stopped = false;
     int up = 0, turns = 0;
     load(x, begin);
-    __syncthreads();                           // a persistent caller's previous block is out of shared memory
-    if (tid == 0) s.line = -INFINITY;
-    __syncthreads();
 #pragma unroll 1
     for (; here < end; here += kBeamTurn) {
         if (flag != nullptr && (++turns & 3) == 0) {       // best-effort flavour: a look at the preempt flag, asked for ahead
@@ -202,15 +187,15 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
             up = ld_flag(flag);
         }
         if (here + kBeamTurn < end) load(next, here + kBeamTurn);
-        float h[kBeamVecs];
+        float high = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kBeamVecs; i++) h[i] = fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w));
-        const float high = fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3]));
+        for (int i = 0; i < kBeamVecs; i++) high = fmaxf(high, fmaxf(fmaxf(x[i].x, x[i].y), fmaxf(x[i].z, x[i].w)));
         if (high > top) {
             const float by = exp2_fast((top - high) * kLog2e);
             sum.x *= by;
             sum.y *= by;
             top = high;
+            turn = here;
         }
         if (top == -INFINITY) {
 #pragma unroll
@@ -225,76 +210,96 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
                 sum = add2(sum, add2(a, b));
             }
         }
-        float line = *(volatile float*)&s.line;        // nothing below it counts, in this warp or another
-        if (here == begin) {
-            int rank = 0;
-#pragma unroll
-            for (int j = 0; j < 32; j++) {
-                const float v = __shfl_sync(0xffffffffu, high, j);
-                rank += v > high || (v == high && j < lane);
-            }
-            line = fmaxf(line, __shfl_sync(0xffffffffu, high, __ffs(__ballot_sync(0xffffffffu, rank == K - 1)) - 1));
-        }
-        // (an equal word of this warp's later turns is too late; among one turn's, and another warp's, it need not be)
-        auto counts = [&](float v, int w) { return v >= line && v > -INFINITY && beam_before(v, w, last, last_i); };
-        if (__any_sync(0xffffffffu, high >= line && high > -INFINITY && high >= last)) {
-            const float before = last;
-#pragma unroll
-            for (int i = 0; i < kBeamVecs; i++) {
-                if (!__any_sync(0xffffffffu, h[i] >= line && h[i] >= last)) continue;
-                const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                const int w = here + (i * 32 + lane) * 4;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    unsigned m = __ballot_sync(0xffffffffu, counts(v[e], w + e));
-                    while (m) {
-                        const int src = __ffs(m) - 1;
-                        move_in(__shfl_sync(0xffffffffu, v[e], src), __shfl_sync(0xffffffffu, w + e, src));
-                        m &= m - 1;
-                        m &= __ballot_sync(0xffffffffu, counts(v[e], w + e));
-                    }
-                }
-            }
-            if (lane == 0 && last > before && last > line) raise(last);
-        }
 #pragma unroll
         for (int i = 0; i < kBeamVecs; i++) x[i] = next[i];
     }
-    // the warps' sums and candidates meet
-    float high = warp_max(top);
-    const float part_sum = sum.x + sum.y, total = warp_sum(top == -INFINITY ? part_sum : part_sum * exp2_fast((top - high) * kLog2e));
+    // the warps' sums and their groups' maxima meet
+    const float high = warp_max(top), part_sum = sum.x + sum.y;
+    const float total = warp_sum(top == -INFINITY ? part_sum : part_sum * exp2_fast((top - high) * kLog2e));
+    const int groups = K <= 8 ? 16 : 32;
+    float key = top;
+    int key_turn = turn;
+    if (groups == 16) {
+        const float v = __shfl_xor_sync(0xffffffffu, key, 16);
+        const int i = __shfl_xor_sync(0xffffffffu, key_turn, 16);
+        if (beam_before(v, i, key, key_turn)) key = v, key_turn = i;
+    }
+    __syncthreads();                           // a persistent caller's previous block is out of shared memory
     if (lane == 0) {
         s.top[warp] = high;
         s.sum[warp] = total;
     }
-    if (lane < K) {
-        s.value[warp][lane] = mine;
-        s.index[warp][lane] = mine_i;
+    if (lane < groups) {
+        s.key[warp][lane] = key;
+        s.turn[warp][lane] = key_turn;
     }
+    if (tid == 0) s.room.count = 0;
     if (__syncthreads_or(stopped)) return false;
-    if (tid == 0) {
-        float all = 0.f;
-        for (int w = 0; w < 8; w++) high = fmaxf(high, s.top[w]);
-        for (int w = 0; w < 8; w++) all += s.top[w] == -INFINITY ? s.sum[w] : s.sum[w] * exp2_fast((s.top[w] - high) * kLog2e);
-        out[0] = high;
-        out[1] = all;
-    }
-    if (tid < 8 * K) {
-        // a candidate's place: how many come before it; those that are none stand behind them, the lowest first
-        const int w = tid / K, c = tid - w * K, index = s.index[w][c];
-        const float v = s.value[w][c];
-        int at = 0;
-#pragma unroll
-        for (int o = 0; o < 8; o++)
-            for (int k = 0; k < K; k++) {
-                const float u = s.value[o][k];
-                const int i = s.index[o][k];
-                at += beam_before(u, i, v, index) || (u == v && i == index && o * K + k < tid);
-            }
-        if (at < K) {
-            out[2 + at] = v;
-            out[2 + K + at] = __int_as_float(index);
+    if (warp == 0) {
+        const float most_of = lane < 8 ? s.top[lane] : -INFINITY, most = warp_max(most_of);
+        const float all = warp_sum(lane >= 8 ? 0.f : most_of == -INFINITY ? s.sum[lane] : s.sum[lane] * exp2_fast((most_of - most) * kLog2e));
+        if (lane == 0) {
+            out[0] = most;
+            out[1] = all;
         }
+    }
+    // the line, by every warp for itself: a group to a lane
+    const int group = lane & (groups - 1);
+    key = s.key[0][group];
+    key_turn = s.turn[0][group];
+#pragma unroll
+    for (int w = 1; w < 8; w++) {
+        const float v = s.key[w][group];
+        const int i = s.turn[w][group];
+        if (beam_before(v, i, key, key_turn)) key = v, key_turn = i;
+    }
+    int rank = 0;
+#pragma unroll 2
+    for (int j = 0; j < groups; j++) {
+        const float v = __shfl_sync(0xffffffffu, key, j);
+        const int i = __shfl_sync(0xffffffffu, key_turn, j);
+        rank += beam_before(v, i, key, key_turn) || (v == key && i == key_turn && j < group);
+    }
+    const int at = __ffs(__ballot_sync(0xffffffffu, rank == K - 1)) - 1;
+    const float line = __shfl_sync(0xffffffffu, key, at);
+    const int line_turn = __shfl_sync(0xffffffffu, key_turn, at), upto = line == -INFINITY ? -0x7fffffff : line_turn + kBeamTurn;
+    const unsigned reach = __ballot_sync(0xffffffffu, top > line || (top == line && turn < upto));
+    auto each = [&](auto f) {                  // eight lanes to one that reaches the line
+        for (unsigned m = reach; m;) {
+            unsigned of = m;
+            for (int j = lane >> 3; j > 0; j--) of &= of - 1;
+            for (int j = 0; j < 4; j++) m &= m - 1;
+            if (of == 0) continue;
+#pragma unroll 1
+            for (int w = begin + (__ffs(of) - 1 + (lane & 7) * 32) * 4; w < end; w += 8 * 8 * 32 * 4) {
+                float4 y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = load_at(w + i * 8 * 32 * 4, end);
+                unsigned some = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) some |= (fmaxf(fmaxf(y[i].x, y[i].y), fmaxf(y[i].z, y[i].w)) >= line) << i;
+                for (; some; some &= some - 1) {       // (few: a short loop over what is in L1 costs less than the code for all eight)
+                    const int at = w + (__ffs(some) - 1) * 8 * 32 * 4;
+                    const float4 z = load_at(at, end);
+                    const float v[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (v[e] > line || (v[e] == line && at + e < upto)) f(v[e], at + e);
+                }
+            }
+        }
+    };
+    auto take = [&](int i, float v, int w) {
+        out[2 + i] = v;
+        out[2 + K + i] = __int_as_float(w);
+    };
+    block_collect<float>(s.room, each);
+    __syncthreads();
+    const int n = s.room.count;
+    const int found = n <= kBeamRoom ? block_place<float>(K, s.room, n, take) : block_top<float>(K, s.room, each, take);
+    if (tid >= found && tid < K) {
+        out[2 + tid] = -INFINITY;
+        out[2 + K + tid] = __int_as_float(0);
     }
     return true;
 }

@@ -455,6 +455,22 @@ def test_beam_select_of_equal_values(K, V):
         check_beams(logits, score, live, K, 1)
 
 
+@pytest.mark.parametrize("Q,K", [(75, 8), (40, 16)])
+def test_beam_select_of_words_in_few_places(Q, K):
+    """Words that stand where few threads look, more than are ranked side by side; words in order."""
+    V, R = 20000, Q * K
+    w = torch.arange(V, device="cuda")
+    logits = torch.where(w // 4 % 16 == 3, torch.randn(R, V, device="cuda"), -torch.inf)
+    logits[K:2 * K, w // 4 % 16 == 3] = 5.0             # all of them equal
+    logits[2 * K:3 * K] = torch.where(w // 4 % 16 == 3, 5.0, torch.finfo(F).min)
+    logits[3 * K:4 * K] = torch.where(w // 4 % 16 < 7, w % 5000 / 1000, -torch.inf)
+    logits[4 * K:5 * K] = w / 1000
+    logits[5 * K:6 * K] = -w / 1000
+    logits[6 * K:7 * K] = torch.where(w > V - 30, 1.0, torch.where(w % 128 < 64, 2.0, 0.0))
+    logits[7 * K:8 * K] = torch.where((w // 4 % 32 == 9) | (w % 1999 == 0), 2.0 + w % 3, -1.0)
+    check_beams(logits, -torch.rand(R, device="cuda"), torch.ones(R, device="cuda", dtype=I), K, 2)
+
+
 @pytest.mark.parametrize("V", [5, 10001])
 def test_beam_select_of_masked_words_and_rows(V):
     K = 4
