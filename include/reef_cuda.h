@@ -218,7 +218,8 @@ REEF_API reef_status reef_dispatch(reef_kernel_t rt, void** rt_args,
  *  - The first call on a device looks up the array's device address (cudaGetSymbolAddress, with that device
  *    current); make that first call before any stream capture begins.
  *  - Logical-block kernels only (one persistent grid); a tensor-core cluster kernel, or another one that is
- *    launched on its own (attrs.tensor_core), on either side is refused with REEF_FAIL.  Everything else is as in reef_dispatch's single-grid form. */
+ *    launched on its own (attrs.tensor_core), on either side is refused with REEF_FAIL.  Everything else is as
+ *    in reef_dispatch's single-grid form. */
 #define REEF_STATIC_DISPATCH_LANES 64
 REEF_API reef_status reef_dispatch_static(reef_kernel_t rt, void** rt_args,
                                           reef_kernel_t be, void** be_args,

@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "simple.cuh"
 
 namespace reef {
@@ -51,7 +53,9 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // 23 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them).
 constexpr int kTablesThreads = 2 * kThreads;
 constexpr int kTablesMaxRows = 1024, kTablesMaxPages = 1 << 19;
-__host__ __device__ constexpr int tables_fixed(int rows, int pages) { return (4 * ((pages + 31) / 32 + 8 * rows + 2 + 96 + kTablesThreads) + 15) / 16 * 16; }
+__host__ __device__ constexpr int tables_fixed(int rows, int pages) {
+    return (4 * ((pages + 31) / 32 + 8 * rows + 2 + 96 + kTablesThreads) + 15) / 16 * 16;
+}
 __host__ __device__ constexpr int tables_window(int rows, int pages) {      // what fits an SM beside the rest
     const int all = (pages + 31) / 32 * 32, room = (225 * 1024 - tables_fixed(rows, pages)) / 512 * 512;
     return all < room ? all : room;
@@ -59,7 +63,7 @@ __host__ __device__ constexpr int tables_window(int rows, int pages) {      // w
 __host__ constexpr int tables_smem(int rows, int pages) { return tables_fixed(rows, pages) + tables_window(rows, pages); }
 constexpr int kTablesSmemMax = 225 * 1024;
 // Twice the threads from 8192 ids on: 64 rows of 512 ids 12.4 us instead of 14.4, 256 rows of 1024 22.7 instead of 26.8, 16 rows of 64
-// 11.2 instead of 10.4.  1024 threads do less, their barriers and sums cost more than they divide: 16.5, 24.3 and 12.4.  A dispatcher's
+// 10.4 instead of 9.0.  1024 threads do less, their barriers and sums cost more than they divide: 16.5, 24.3 and 12.4.  A dispatcher's
 // blocks, which have kThreads, do the same work.
 __host__ inline int tables_threads(int rows, int max_pages) { return (long long)rows * max_pages >= 8192 ? kTablesThreads : kThreads; }
 // Rows and tokens are written by up to 32 blocks, 4096 ids or 256 tokens to a block.
@@ -187,13 +191,13 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                     if (left <= 128 && len[row] != kept(row) * S) left |= 1 << 30;     // its last id names a page that is written
                 }
                 const int n = min(32, (all1[0] - c0 - warp + warps - 1) / warps);
-#pragma unroll 1
-                for (int i0 = 0; i0 < n; i0 += 8) {
-                    int4 id[8];
-                    int count[8];
+                auto look = [&](auto at_once, int i0) {
+                    constexpr int P = decltype(at_once)::value;
+                    int4 id[P];
+                    int count[P];
                     unsigned ill = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < P; i++) {
                         const int* from4 = table + __shfl_sync(0xffffffffu, at, i0 + i) + 4 * lane;
                         count[i] = __shfl_sync(0xffffffffu, left, i0 + i);       // (0 behind the last piece)
                         const int m = min(count[i] & ~(1 << 30), 128) - 4 * lane;
@@ -209,7 +213,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < P; i++) {
                         const int m = min(count[i] & ~(1 << 30), 128) - 4 * lane, written = count[i] & (1 << 30) ? m - 1 : -1;
                         const int v[4] = {id[i].x, id[i].y, id[i].z, id[i].w};
 #pragma unroll
@@ -222,12 +226,16 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                     if (__any_sync(0xffffffffu, ill)) {
                         wrong = true;
 #pragma unroll 1
-                        for (int i = 0; i < 8; i++) {
+                        for (int i = 0; i < P; i++) {
                             const int r = __shfl_sync(0xffffffffu, row, i0 + i);
                             if (__any_sync(0xffffffffu, ill >> i & 1) && lane == 0) bad[from[r]] = 1;
                         }
                     }
-                }
+                };
+                if (n <= 2) look(std::integral_constant<int, 2>(), 0);        // (little code: it is fetched for one use)
+                else
+#pragma unroll 1
+                    for (int i0 = 0; i0 < n; i0 += 8) look(std::integral_constant<int, 8>(), i0);
             }
             __syncthreads();
             for (int w = tid; w < window / 32 && first / 32 + w < words; w += threads) {
