@@ -50,7 +50,7 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // Used pages are marked in bytes, a window of the pages at a time, and packed to bits: an atomic OR into a word of bits took 1.5 cycles for
 // every id, 53 us for 62500 of them, a byte is a plain store.  A free page is found by its rank (a prefix sum over the threads' words, a walk
 // through one thread's), by whoever needs it.  16 rows of 500 tokens 7 us, 128 beams 12, 256 rows of two million tokens in all (62500 ids)
-// 23 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them).
+// 21 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them).
 constexpr int kTablesThreads = 2 * kThreads;
 constexpr int kTablesMaxRows = 1024, kTablesMaxPages = 1 << 19;
 __host__ __device__ constexpr int tables_fixed(int rows, int pages) {
@@ -62,8 +62,8 @@ __host__ __device__ constexpr int tables_window(int rows, int pages) {      // w
 }
 __host__ constexpr int tables_smem(int rows, int pages) { return tables_fixed(rows, pages) + tables_window(rows, pages); }
 constexpr int kTablesSmemMax = 225 * 1024;
-// Twice the threads from 8192 ids on: 64 rows of 512 ids 12.4 us instead of 14.4, 256 rows of 1024 22.7 instead of 26.8, 16 rows of 64
-// 10.4 instead of 9.0.  1024 threads do less, their barriers and sums cost more than they divide: 16.5, 24.3 and 12.4.  A dispatcher's
+// Twice the threads from 8192 ids on: 64 rows of 512 ids 12.4 us instead of 14.4, 256 rows of 1024 20.6 instead of 26.8, 16 rows of 64
+// 10.4 instead of 9.0.  With 1024 threads barriers and sums cost more than is divided: 16.5, 24.3 and 12.4.  A dispatcher's
 // blocks, which have kThreads, do the same work.
 __host__ inline int tables_threads(int rows, int max_pages) { return (long long)rows * max_pages >= 8192 ? kTablesThreads : kThreads; }
 // Rows and tokens are written by up to 32 blocks, 4096 ids or 256 tokens to a block.
@@ -214,14 +214,20 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                     }
 #pragma unroll
                     for (int i = 0; i < P; i++) {
-                        const int m = min(count[i] & ~(1 << 30), 128) - 4 * lane, written = count[i] & (1 << 30) ? m - 1 : -1;
-                        const int v[4] = {id[i].x, id[i].y, id[i].z, id[i].w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int x = e < m ? v[e] : -1;
-                            if (x < -1 || x >= N || (x < 0 && e == written)) ill |= 1u << i;
-                            if (x >= first && x - first < window) mark[x - first] = 1;
+                        const int m = min(count[i] & ~(1 << 30), 128) - 4 * lane;
+                        int4 x = id[i];
+                        if (m > 0 && m <= 4) {                        // the row's last ids, or the piece's
+                            const int end = m == 1 ? x.x : m == 2 ? x.y : m == 3 ? x.z : x.w;
+                            if (count[i] >> 30 && end < 0) ill |= 1u << i;
+                            if (m < 2) x.y = -1;
+                            if (m < 3) x.z = -1;
+                            if (m < 4) x.w = -1;
                         }
+                        if (max(max(x.x, x.y), max(x.z, x.w)) >= N || min(min(x.x, x.y), min(x.z, x.w)) < -1) ill |= 1u << i;
+                        const unsigned at[4] = {(unsigned)x.x - first, (unsigned)x.y - first, (unsigned)x.z - first, (unsigned)x.w - first};
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (at[e] < (unsigned)window) mark[at[e]] = 1;
                     }
                     if (__any_sync(0xffffffffu, ill)) {
                         wrong = true;
