@@ -307,7 +307,7 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
 // ---- pick: the parts of a request's beams -> its new beams --------------------------------------------------------------------
 // args: parts, score, live, [start], token, parent, score', live'.  Within a beam the logits decide, exactly as they are; beams are
 // compared in 64 bits: a score of -50 in 32 bits cannot tell logits apart that differ by less than 4e-6.  Latency: 32 requests of eight beams
-// 8 us.
+// 6 us, an entry of a list to a thread (8 with a list to a thread).
 __host__ inline int beam_pick_smem() { return kBeamSmem + kBeamMax * (8 + 8 + 4 + 4); }
 __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned char* smem, const int*) {
     const BeamP& p = t.p.beam;
@@ -357,19 +357,16 @@ __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned 
         }
     }
     __syncthreads();
-    const int lists = K * p.parts;
+    const int entries = K * p.parts * K;
     const int found = block_top<double>(K, s,
         [&](auto f) {
-            for (int c = tid; c < lists; c += kThreads) {
-                const int b = c / p.parts;
-                if (kind[b] != 1) continue;
-                const float* x = parts + (size_t)c * F;
-                for (int i = 0; i < K; i++) {
-                    const float v = x[2 + i];
-                    const int w = __float_as_int(x[2 + K + i]);
-                    if (v == -INFINITY) break;
-                    f((double)v - highest[b] - log_sum[b] + base[b], b * p.vocab + min(max(w, 0), p.vocab - 1));
-                }
+#pragma unroll 2
+            for (int c = tid; c < entries; c += kThreads) {
+                const int list = c / K, b = list / p.parts;
+                const float* x = parts + (size_t)list * F + 2 + (c - list * K);
+                const float v = x[0];
+                const int w = __float_as_int(x[K]);
+                if (kind[b] == 1) f((double)v - highest[b] - log_sum[b] + base[b], b * p.vocab + min(max(w, 0), p.vocab - 1));
             }
             if (tid < K && kind[tid] == 2) f((double)score[tid], tid * p.vocab + p.eos);
         },
