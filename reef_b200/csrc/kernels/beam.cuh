@@ -128,9 +128,9 @@ __device__ __forceinline__ int beam_logits(const BeamP& p, const int* start, int
 // are divided into 16 groups, or 32 for more beams than 8, whose words lie all over the part.  K groups have a word at or above the K-th
 // greatest of their maxima, so nothing but what reaches that line (words above it, and those equal to it up to its turn) can be among
 // the K greatest.  The words of the lanes whose maxima reach it, some 12 of 256, are read again, from L2, and those that do are ranked.
-// 256 rows of 100003 words, 102 MB, 23 us (0.70 of the measured copy rate; 39 with the greatest words kept in order as they came, 61 with a room
-// in shared memory that was ranked whenever it filled), of these 19 for the pass and the rest for the line, the second look and the ranking,
-// during which nothing is read; four rows of 30522 words 6.  Code of many unrolled steps after the pass is itself slow, every line of
+// 256 rows of 100003 words, 102 MB, 26 us from HBM (0.60 of the measured copy rate), 23 with most of it in L2 (39 with the greatest words kept in
+// order as they came, 61 with a room in shared memory that was ranked whenever it filled); 22 and 19 of these are the pass, the rest the
+// line, the second look and the ranking, during which little is read; four rows of 30522 words 6.  Code of many unrolled steps after the pass is itself slow, every line of
 // it being fetched once: a loop unrolled 16 times took 1 us longer than the loop.
 struct BeamScan {
     BeamRoom<float> room;
