@@ -14,7 +14,7 @@
 
 namespace reef {
 
-constexpr int kThreads = 256;   // every family runs 256-thread blocks so the dispatcher can host any of them
+constexpr int kThreads = 256;   // threads of a dispatcher's block: every family that it hosts can run with them
 constexpr int kMaxArgs = 10;
 
 enum Family : int {
