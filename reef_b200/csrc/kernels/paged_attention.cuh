@@ -844,6 +844,15 @@ __host__ inline int paged_heads_of_a_pass(int kt, int d, int group) {
     const int most = d == 256 ? 4 : 8, passes = (group + most - 1) / most, gb = (group + passes - 1) / passes;
     return gb == 7 ? 8 : gb;
 }
+// Warps of a pass where no parts are left: a second, fourth or eighth shortens a pass, and costs a join and, where there are passes enough for
+// all warps, further rounds of blocks.  Measured in 1, 2, 4 and 8 warps (us): 2048 passes of up to 8 units 24.6, 30.8, 35.5, 45.2; 16 units
+// 29.9, 33.2, 35.9, 45.1; 32 units 73.9, 73.4, 69.6, 78.4; 128 units 266, 230, 203, 197; 512 passes of 8 units 16.6, 14.5, 12.4, 15.1, of 32 units
+// 49, 30.9, 24.2, 26.1; 384 of 32 units 20.6, 16.6, 12.4, 12.4.  So as many as it takes to have 1536 warps, or no more than 16 units a warp.
+__host__ inline int paged_warps_of_a_pass(long long passes, int units) {
+    int w = 1;
+    while (w < 8 && w < units && (passes * w < 1536 || units > 16 * w)) w *= 2;
+    return w;
+}
 __host__ inline bool paged_mma(const PagedP& p) { return p.kt != KT_FP32 && p.gb > 2; }
 struct PagedSimtShape { int unit, scratch; };
 __host__ inline PagedSimtShape paged_simt_shape(const PagedP& p) {      // UNIT and SCRATCH of PagedSimt

@@ -383,7 +383,14 @@ constexpr int kAppendPerBlock = 4 * kThreads * 4;       // fp32 values of k, and
 __host__ inline int append_token_blocks(const PagedP& p) {
     return (int)(((long long)p.tokens * p.kvh * p.d + kAppendPerBlock - 1) / kAppendPerBlock);
 }
-__host__ inline int append_fork_blocks(const PagedP& p) { return p.has_fork ? (p.rows * p.kvh + 3) / 4 : 0; }
+// A fork's page is copied in pieces of 8 KB, a warp to one of keys or values: one warp for a whole page of 64 KB took 65 us.
+constexpr int kForkPiece = 8192;
+__host__ __device__ inline int append_fork_pieces(const PagedP& p) {
+    return (p.ps * p.d * (p.kt == KT_FP32 ? 4 : 2) + kForkPiece - 1) / kForkPiece;
+}
+__host__ inline long long append_fork_blocks(const PagedP& p) {
+    return p.has_fork ? ((long long)p.rows * p.kvh * append_fork_pieces(p) + 3) / 4 : 0;
+}
 
 __device__ __forceinline__ void store4(float* at, float4 x) { *reinterpret_cast<float4*>(at) = x; }
 __device__ __forceinline__ void store4(__nv_bfloat16* at, float4 x) {
@@ -439,20 +446,28 @@ __device__ __forceinline__ bool body_paged_append(const KTask& t, int vb, unsign
         else append_tokens<__half>(p, t, vb);
         return true;
     }
-    // forks: two warps to a head of a forked page, one for keys and one for values
+    // forks: two warps to a piece of a head's forked page, one for keys and one for values
     const int4* fork = (const int4*)t.a[3];
-    const int item = (vb - p.split) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 31;
-    if (item >= p.rows * p.kvh) return true;
-    const int r = item / p.kvh, h = item - r * p.kvh;
+    const int pieces = append_fork_pieces(p), item = (vb - p.split) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 31;
+    const int of = item / pieces, r = of / p.kvh, h = of - r * p.kvh;
+    if (r >= p.rows) return true;
     const int4 c = fork[r];
     if ((unsigned)c.x >= (unsigned)p.pages || (unsigned)c.y >= (unsigned)p.pages || c.x == c.y) return true;
-    const int e = p.kt == KT_FP32 ? 4 : 2, words = min(c.z, p.ps) * (p.d * e / 16);
+    const int e = p.kt == KT_FP32 ? 4 : 2, from = (item - of * pieces) * (kForkPiece / 16);
+    const int words = min(min(c.z, p.ps) * (p.d * e / 16), from + kForkPiece / 16);
     const size_t page = (size_t)p.ps * p.d * e;
     char* cache = (char*)t.a[threadIdx.x & 32 ? 5 : 4];
     const uint4* src = (const uint4*)(cache + ((size_t)c.x * p.kvh + h) * page);
     uint4* dst = (uint4*)(cache + ((size_t)c.y * p.kvh + h) * page);
-#pragma unroll 4
-    for (int i = lane; i < words; i += 32) dst[i] = src[i];
+    for (int i = from + lane; i < words; i += 32 * 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + 32 * k < words) x[k] = src[i + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + 32 * k < words) dst[i + 32 * k] = x[k];
+    }
     return true;
 }
 

@@ -159,7 +159,8 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
         if ((long long)p.rows * p.kvh > (1 << 30) || (long long)p.tokens * row > 0x70000000LL) return false;
         p.split = append_token_blocks(p);
         t.family = F_PAGED_APPEND;
-        t.nblocks = p.split + append_fork_blocks(p);
+        if (append_fork_blocks(p) + p.split > (1 << 28)) return false;
+        t.nblocks = p.split + (int)append_fork_blocks(p);
         s->nargs = p.has_fork ? 6 : 5;
         s->bytes = 2.0 * p.tokens * row * (4.0 + cache_bytes(p.kt)) + 16.0 * (p.tokens + p.rows);
         return true;
@@ -200,7 +201,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
         t.nblocks = blocks;
         s->nargs = 7;
     } else {
-        p.wpp = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
+        p.wpp = paged_warps_of_a_pass(passes, units);
         t.nblocks = (int)((passes * p.wpp + 7) / 8);
         s->nargs = 6;
     }

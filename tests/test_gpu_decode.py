@@ -215,6 +215,12 @@ def test_append(type, T, kv, D, S, pages, forks, stride):
         assert all(torch.equal(a, b) for a, b in zip(caches, want))
 
 
+@pytest.mark.parametrize("type", [F, torch.bfloat16])
+def test_append_copies_pages_of_several_pieces(type):
+    test_append(type, 20, 3, 256, 100, 40, 7, 0)
+    test_append(type, 2, 1, 128, 128, 9, 4, 0)
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------------
 def attend_by_hand(q, kc, vc, table, tok):
     """(result, sum p |v|) in 64 bits"""
@@ -291,6 +297,17 @@ def test_attention(type, D, H, kv, M, S, lens):
 def test_attention_page_sizes(S, type):
     M = -(-1300 // S)
     check_attention(*attend_inputs(np.random.default_rng(S), [1300 // S * S, 1, S, min(S + 1, M * S), 777], 6, 3, 64, S, M, type))
+
+
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("D,H,kv", [(64, 16, 16), (128, 24, 8), (256, 16, 8), (64, 40, 8)])
+def test_attention_of_many_short_rows(type, D, H, kv):
+    """Passes enough for all warps: one, two or four warps to a pass, rows without keys and of one key among them."""
+    for R, M in ((90, 2), (200, 3), (130, 9)):
+        rng = np.random.default_rng([R, D, H])
+        lens = rng.integers(-1, M * 16 + 3, R)
+        lens[rng.random(R) < 0.2] = 1
+        check_attention(*attend_inputs(rng, lens, H, kv, D, 16, M, type))
 
 
 @pytest.mark.parametrize("type", TYPES)
