@@ -62,16 +62,13 @@ __device__ __forceinline__ int block_place(int K, const BeamRoom<V>& s, int n, T
     }
     return min(n, K);
 }
-// Every warp's K-th greatest of its lanes' maxima has K values at or above it, so the greatest of these eight is a line that few values
-// reach.  Where more reach it than there is room for (many equal values) the best one behind the last is looked for K times.
-template <class V, class Each, class Take>
-__device__ __forceinline__ int block_top(int K, BeamRoom<V>& s, Each each, Take take) {
+// Every warp's K-th greatest of its lanes' values has K values at or above it, so the greatest of these eight is a line that few values reach.
+// (s.count is 0 behind it.)
+template <class V>
+__device__ __forceinline__ V block_line(int K, BeamRoom<V>& s, V top) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const V ninf = -INFINITY;
-    V top = ninf;
-    each([&](V v, int) { if (v > top) top = v; });
     int rank = 0;
-#pragma unroll
+#pragma unroll 4
     for (int j = 0; j < 32; j++) {
         const V v = __shfl_sync(0xffffffffu, top, j);
         rank += v > top || (v == top && j < lane);
@@ -83,6 +80,16 @@ __device__ __forceinline__ int block_top(int K, BeamRoom<V>& s, Each each, Take 
     V line = s.line[0];
 #pragma unroll
     for (int w = 1; w < 8; w++) line = s.line[w] > line ? s.line[w] : line;
+    return line;
+}
+// The line is drawn through the threads' maxima.  Where more reach it than there is room for (many equal values) the best one behind the last is looked for K times.
+template <class V, class Each, class Take>
+__device__ __forceinline__ int block_top(int K, BeamRoom<V>& s, Each each, Take take) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const V ninf = -INFINITY;
+    V top = ninf;
+    each([&](V v, int) { if (v > top) top = v; });
+    const V line = block_line<V>(K, s, top);
     block_collect<V>(s, [&](auto f) { each([&](V v, int i) { if (v >= line) f(v, i); }); });
     __syncthreads();
     const int n = s.count;
@@ -307,8 +314,10 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
 // ---- pick: the parts of a request's beams -> its new beams --------------------------------------------------------------------
 // args: parts, score, live, [start], token, parent, score', live'.  Within a beam the logits decide, exactly as they are; beams are
 // compared in 64 bits: a score of -50 in 32 bits cannot tell logits apart that differ by less than 4e-6.  Latency: 32 requests of eight beams
-// 6 us, an entry of a list to a thread (8 with a list to a thread).
-__host__ inline int beam_pick_smem() { return kBeamSmem + kBeamMax * (8 + 8 + 4 + 4); }
+// 6 us, one of sixteen beams in 25 parts each 14 (141 when every entry was looked at: the lists are in order, and a line through threads that have
+// entries of every rank is a low one).
+constexpr int kBeamLists = 4 * 148 + kBeamMax;            // lists of a request at most: parts of all rows, or one of each
+__host__ inline int beam_pick_smem() { return kBeamSmem + kBeamMax * (8 + 8 + 4 + 4) + kBeamLists * (8 + 4) + 8; }
 __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned char* smem, const int*) {
     const BeamP& p = t.p.beam;
     const int K = p.beams, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, F = beam_part_floats(K);
@@ -328,6 +337,9 @@ __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned 
     double* base = log_sum + kBeamMax;
     float* highest = reinterpret_cast<float*>(base + kBeamMax);
     int* kind = reinterpret_cast<int*>(highest + kBeamMax);           // 0: no candidates, 1: its parts, 2: it has ended
+    double* heads = reinterpret_cast<double*>(kind + kBeamMax);       // the lists' first entries
+    int* which = reinterpret_cast<int*>(heads + kBeamLists);          // lists that reach the line
+    int* walked = which + kBeamLists;                                 // how many
     __syncthreads();
     for (int b = warp; b < K; b += 8) {
         const int r = vb * K + b;
@@ -357,26 +369,56 @@ __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned 
         }
     }
     __syncthreads();
-    const int entries = K * p.parts * K;
-    const int found = block_top<double>(K, s,
-        [&](auto f) {
+    // a list's i-th entry: the value, -infinity for none, and the place among the request's candidates
+    const int lists = K * p.parts;
+    auto entry = [&](int list, int i, int* at) -> double {
+        const int b = list / p.parts;
+        const float* x = parts + (size_t)list * F + 2 + i;
+        const float v = x[0];
+        *at = b * p.vocab + min(max(__float_as_int(x[K]), 0), p.vocab - 1);
+        return kind[b] == 1 ? (double)v - highest[b] - log_sum[b] + base[b] : -INFINITY;
+    };
+    auto take = [&](int i, double v, int at) {
+        const int b = at / p.vocab, w = at - b * p.vocab;
+        token[i] = w;
+        parent[i] = vb * K + b;
+        score_out[i] = (float)v;
+        live_out[i] = kind[b] == 1 && w != p.eos;
+    };
+    // K first entries reach the line: only lists whose first entries do are looked into
+    const double own = tid < K && kind[tid] == 2 ? (double)score[tid] : -INFINITY;
+    double top = own;
+    int at;
+    for (int c = tid; c < lists; c += kThreads) {
+        heads[c] = entry(c, 0, &at);
+        top = fmax(top, heads[c]);
+    }
+    if (tid == 0) *walked = 0;
+    const double line = block_line<double>(K, s, top);
+    for (int c = tid; c < lists; c += kThreads)
+        if (heads[c] >= line && heads[c] > -INFINITY) which[atomicAdd(walked, 1)] = c;
+    __syncthreads();
+    const int entries = *walked * K;
+    block_collect<double>(s, [&](auto f) {
 #pragma unroll 2
-            for (int c = tid; c < entries; c += kThreads) {
-                const int list = c / K, b = list / p.parts;
-                const float* x = parts + (size_t)list * F + 2 + (c - list * K);
-                const float v = x[0];
-                const int w = __float_as_int(x[K]);
-                if (kind[b] == 1) f((double)v - highest[b] - log_sum[b] + base[b], b * p.vocab + min(max(w, 0), p.vocab - 1));
+        for (int c = tid; c < entries; c += kThreads) {
+            const int list = c / K;
+            const double v = entry(which[list], c - list * K, &at);
+            if (v >= line) f(v, at);
+        }
+        if (own >= line) f(own, tid * p.vocab + p.eos);
+    });
+    __syncthreads();
+    const int n = s.count;
+    const int found = n <= kBeamRoom ? block_place<double>(K, s, n, take) : block_top<double>(K, s,
+        [&](auto f) {
+            for (int c = tid; c < lists * K; c += kThreads) {
+                const int list = c / K;
+                const double v = entry(list, c - list * K, &at);
+                f(v, at);
             }
-            if (tid < K && kind[tid] == 2) f((double)score[tid], tid * p.vocab + p.eos);
-        },
-        [&](int i, double v, int at) {
-            const int b = at / p.vocab, w = at - b * p.vocab;
-            token[i] = w;
-            parent[i] = vb * K + b;
-            score_out[i] = (float)v;
-            live_out[i] = kind[b] == 1 && w != p.eos;
-        });
+            f(own, tid * p.vocab + p.eos);
+        }, take);
     if (tid >= found && tid < K) {
         token[tid] = -1;
         parent[tid] = -1;
