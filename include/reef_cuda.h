@@ -156,7 +156,7 @@ typedef struct {
     double flops;          /* algorithmic FLOPs of one launch                               */
     double bytes;          /* algorithmic HBM bytes of one launch                           */
     int tensor_core;       /* 1 when the kernel's contraction runs on tcgen05, or it is otherwise a kernel of
-                              its own that the dispatcher does not host (a block to half an SM) */
+                              its own that the dispatcher does not host (a block to an SM or half of one) */
     int cluster;           /* thread blocks per cluster (1 = no cluster); block ranges handed to
                               reef_dispatch for this kernel must be multiples of it           */
     int chainable;         /* 1: a tensor-core convolution / matmul that reef_chain_create accepts */

@@ -40,8 +40,8 @@ struct PagedFns {
     static const void* of(int gb) {
         return gb == 1 ? (const void*)k_paged_attention<PagedSimt<C, D, 1>, 2>
              : gb == 2 ? (const void*)k_paged_attention<PagedSimt<C, D, 2>, 2>
-             : gb == 4 ? (const void*)k_paged_attention<PagedMma<C, D, 4>, D == 256 ? 1 : 2>
-             : gb == 8 ? (const void*)k_paged_attention<PagedMma<C, D, 8>, D == 256 ? 1 : 2> : nullptr;
+             : gb == 4 ? (const void*)k_paged_attention<PagedMma<C, D, 4>, 1>
+             : gb == 8 ? (const void*)k_paged_attention<PagedMma<C, D, 8>, 1> : nullptr;
     }
 };
 template <int D, int GB>

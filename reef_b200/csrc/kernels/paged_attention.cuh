@@ -70,9 +70,11 @@ struct PagedRow {
 // How keys and values reach a warp: a step's keys, its values, the next step's keys ... go through a ring of RING stages of its own in
 // shared memory by cp.async, RING - 1 of them under way.  A warp's request covers 512 bytes that lie together in memory: lanes that fetched
 // the pieces they use themselves, 32 bytes of every row, had half of the bandwidth (3.7 instead of 6.8 TB/s from tiles of 4 KB).
-// Stages of a ring: as many as two blocks find room for on an SM, with 256 dimensions on the tensor cores one block.
+// Stages of a ring: as many as the blocks of an SM find room for, two with fp32 instructions, one on the tensor cores.  There the operands do
+// not fit 128 registers, and fewer warps with more under way each leave fewer parts and less to join: a row of 131072 keys 34 and 8 us with two
+// blocks to an SM and 3 stages, 30 and 6 with one block and 6; 90 rows of 48 heads over 6 75 and 65, of 24 heads 58 and 59.
 constexpr int kPagedSimtRing = 6;
-__host__ __device__ constexpr int paged_mma_ring(int d) { return d == 64 ? 6 : 3; }
+__host__ __device__ constexpr int paged_mma_ring(int d) { return 768 / d; }
 // (a range that is worked out again needs its slot and a ring of its own)
 __host__ __device__ constexpr int paged_mma_scratch(int d, int heads) {
     const int ring = paged_mma_ring(d) * d * 32, again = heads * paged_stride(d) * 4 + 4 * 2048;
@@ -844,15 +846,6 @@ __host__ inline int paged_heads_of_a_pass(int kt, int d, int group) {
     const int most = d == 256 ? 4 : 8, passes = (group + most - 1) / most, gb = (group + passes - 1) / passes;
     return gb == 7 ? 8 : gb;
 }
-// Warps of a pass where no parts are left: a second, fourth or eighth shortens a pass, and costs a join and, where there are passes enough for
-// all warps, further rounds of blocks.  Measured in 1, 2, 4 and 8 warps (us): 2048 passes of up to 8 units 24.6, 30.8, 35.5, 45.2; 16 units
-// 29.9, 33.2, 35.9, 45.1; 32 units 73.9, 73.4, 69.6, 78.4; 128 units 266, 230, 203, 197; 512 passes of 8 units 16.6, 14.5, 12.4, 15.1, of 32 units
-// 49, 30.9, 24.2, 26.1; 384 of 32 units 20.6, 16.6, 12.4, 12.4.  So as many as it takes to have 1536 warps, or no more than 16 units a warp.
-__host__ inline int paged_warps_of_a_pass(long long passes, int units) {
-    int w = 1;
-    while (w < 8 && w < units && (passes * w < 1536 || units > 16 * w)) w *= 2;
-    return w;
-}
 __host__ inline bool paged_mma(const PagedP& p) { return p.kt != KT_FP32 && p.gb > 2; }
 struct PagedSimtShape { int unit, scratch; };
 __host__ inline PagedSimtShape paged_simt_shape(const PagedP& p) {      // UNIT and SCRATCH of PagedSimt
@@ -864,7 +857,18 @@ __host__ inline int paged_unit(const PagedP& p) { return paged_mma(p) ? 16 : pag
 __host__ inline int paged_attention_smem(const PagedP& p) {
     return (int)((sizeof(PagedSlots) + 15) & ~15) + 8 * (paged_mma(p) ? paged_mma_scratch(p.d, p.gb) : paged_simt_shape(p).scratch);
 }
-__host__ inline int paged_blocks_per_sm(const PagedP& p) { return paged_mma(p) && p.d == 256 ? 1 : 2; }
+__host__ inline int paged_blocks_per_sm(const PagedP& p) { return paged_mma(p) ? 1 : 2; }
+// Warps of a pass where no parts are left: a second, fourth or eighth shortens a pass, and costs a join and, where there are passes enough for
+// all warps, further rounds of blocks.  Measured in 1, 2, 4 and 8 warps (us): fp32 instructions, 1536 passes of up to 32 units 26.8, 29.1, 28.2,
+// 32.9, of 128 units 94, 80, 73, 68; 384 of 32 units 20.6, 16.6, 12.4, 12.4; 1832 of 16 units 22, 27, 28, 37.  Tensor cores, 2048 passes of 8 units
+// 22.7, 36.9, 45.1, 65.6; 32 units 66, 72, 80, 102; 128 units 228, 201, 191, 201; 512 passes of 32 units 36.9, 24.7, 24.7, 28.8.  So as many as it
+// takes to have warps for two thirds of the machine, or no more than 16 units a warp, 32 on the tensor cores.
+__host__ inline int paged_warps_of_a_pass(const PagedP& p, long long passes, int units) {
+    const int blocks = paged_blocks_per_sm(p), most = 32 / blocks;
+    int w = 1;
+    while (w < 8 && w < units && (passes * w < 768 * blocks || units > most * w)) w *= 2;
+    return w;
+}
 // Blocks of the form with parts: what the SMs hold at once, fewer where the longest rows would not give every warp its least work.  (SMs do
 // not get the same share of the memory's bandwidth: of 148 equal shares of 860 MB one was through after 107 us and one after 147.  Two or
 // three times as many blocks, to be taken by whichever SM is free, brought 157 to 152 us, and cost more in further parts and their join.)

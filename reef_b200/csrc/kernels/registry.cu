@@ -191,7 +191,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
     if (!maybe_between(a, "qs", 0, 0x7fffffff, p.heads * p.d, &p.qs) || !maybe_between(a, "qo", 0, 0x7fffffff, 0, &p.qo)) return false;
     if ((p.qs | p.qo) & 3 || (p.tokens > 1 && p.qs < p.heads * p.d)) return false;
     t.family = F_PAGED_ATTENTION;
-    s->tensor_core = 1;     // launched on its own, a block to half an SM
+    s->tensor_core = 1;     // launched on its own, a block to an SM or to half of one
     s->dyn_smem = (uint32_t)paged_attention_smem(p);
     // the most that a launch can have to do: every row as long as its table
     s->flops = 4.0 * p.tokens * (double)p.heads * p.d * p.mp * p.ps;
@@ -201,7 +201,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
         t.nblocks = blocks;
         s->nargs = 7;
     } else {
-        p.wpp = paged_warps_of_a_pass(passes, units);
+        p.wpp = paged_warps_of_a_pass(p, passes, units);
         t.nblocks = (int)((passes * p.wpp + 7) / 8);
         s->nargs = 6;
     }
