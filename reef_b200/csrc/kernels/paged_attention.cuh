@@ -4,9 +4,9 @@
 // a sequence only, resource/bert/bert.cu:22-157.)
 //
 // One pass over the keys with a running maximum and sum; every key and value is read once for up to eight query heads.  Bound by HBM where
-// there is much to read: 64 rows of 32 heads over 8, bf16, 128 dimensions, 860 MB in 157 us (5.5 TB/s, 0.85 of the measured copy rate; SMs
-// do not get equal shares of it), 2048 passes of up to 2 MB 353 us (0.97); fp32 in groups of five, 188 MB in 41 us (0.70).  A
-// call with little to read is a chain of latencies: 12 heads of a row of 77 keys 5.1 us, of 1000 14.
+// there is much to read: 64 rows of 32 heads over 8, bf16, 128 dimensions, 860 MB in 152 us (5.7 TB/s, 0.88 of the measured copy rate; SMs
+// do not get equal shares of it), 2048 passes of up to 1 MB 185 us (0.89); fp32 in groups of five, 188 MB in 41 us (0.70).  A
+// call with little to read is a chain of latencies: 12 heads of a row of 77 keys 5.0 us, of 1000 14.
 #pragma once
 #include "bf16_split.cuh"
 #include "paged_cache.cuh"

@@ -28,9 +28,10 @@ def paged_attention(tokens: int, rows: int, heads: int, kv_heads: int, dim: int,
 
     One kernel leaves a row's keys to one block per key head: no join, and blocks that wait for a free SM even out what SMs and rows differ by;
     two divide all keys evenly.  Measured (us, one kernel / two, floor; rows of random length up to the longest, whose keys and values of
-    a head are B bytes): 12 heads of one row, B = 512 KB 14.4 / 13.4 for the longest and 6.3 / 12.5 for a short one; 64, 1 MB 27 / 18 (6); 192,
-    512 KB 14.4 / 18, 1 MB 21 / 19 (12); 512, 1 MB 65 / 70 (42); 2048, 2 MB 353 / 383 (343); but 512 of very uneven rows, 4 MB, would wait for
-    the longest.  One kernel, therefore, up to 512 KB and as much again for every 320 heads."""
+    a head are B bytes): 12 heads of all rows, B = 512 KB 14.5 / 13.4 for the longest and 6.3 / 12.5 for a short one; 64, 1 MB 22.7 / 20.8 (6);
+    192, 512 KB 18.6 / 20 (11), 1 MB 30.8 / 33.7 (18), 2 MB 54 / 53 (38); 512, 1 MB 71 / 70 (46); 768, 1 MB 79 / 88 (69), 2 MB 153 / 155 (139); 2048,
+    1 MB 185 / 207 (164); but 512 of very uneven rows, 4 MB, would wait for the longest.  One kernel, therefore, up to 512 KB and as much
+    again for every 320 heads."""
     shape = dict(tokens=tokens, rows=rows, heads=heads, kvh=kv_heads, d=dim, ps=page_size, mp=max_pages, pages=pages, kt=CACHE_TYPES[cache])
     longest = 2 * max_pages * page_size * dim * (4 if cache == "float32" else 2)
     if longest <= (512 << 10) * (1 + tokens * kv_heads / 320):
