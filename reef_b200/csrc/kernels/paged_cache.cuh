@@ -257,6 +257,7 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
                 if (first / 32 + w == words - 1 && (N & 31)) x &= (1u << (N & 31)) - 1;
                 open[first / 32 + w] = x;
             }
+            if (first + window < N) __syncthreads();       // every mark is packed before the next window clears them
         }
         if (!__syncthreads_or(wrong)) break;
         for (int r = tid; r < R; r += threads)
