@@ -822,6 +822,7 @@ __device__ __forceinline__ bool run_body(const KTask& t, int vb, unsigned char* 
 }
 
 // (not inlined: the dispatcher calls it for either kind, and two copies of every body spilled)
+template <bool DECODING>
 __device__ __noinline__ bool run_any(const KTask& t, int vb, unsigned char* smem, const int* flag) {
     switch (t.family) {
         case F_MOCK_ADD: return run_body<F_MOCK_ADD>(t, vb, smem, flag, EnterAlways());
@@ -841,13 +842,19 @@ __device__ __noinline__ bool run_any(const KTask& t, int vb, unsigned char* smem
         case F_LAYERNORM: return run_body<F_LAYERNORM>(t, vb, smem, flag, EnterAlways());
         case F_ATTENTION:           // (the staged form for either: the dispatcher has 128 registers; same results bit for bit)
         case F_ATTENTION_STAGED: return run_body<F_ATTENTION_STAGED>(t, vb, smem, flag, EnterAlways());
-        case F_PAGE_TABLES: return run_body<F_PAGE_TABLES>(t, vb, smem, flag, EnterAlways());
-        case F_PAGED_APPEND: return run_body<F_PAGED_APPEND>(t, vb, smem, flag, EnterAlways());
-        case F_PAGED_JOIN: return run_body<F_PAGED_JOIN>(t, vb, smem, flag, EnterAlways());
-        case F_BEAM_SCAN: return run_body<F_BEAM_SCAN>(t, vb, smem, flag, EnterAlways());
-        case F_BEAM_PICK: return run_body<F_BEAM_PICK>(t, vb, smem, flag, EnterAlways());
-        default: return true;
+        default: break;
     }
+    if (DECODING) {
+        switch (t.family) {
+            case F_PAGE_TABLES: return run_body<F_PAGE_TABLES>(t, vb, smem, flag, EnterAlways());
+            case F_PAGED_APPEND: return run_body<F_PAGED_APPEND>(t, vb, smem, flag, EnterAlways());
+            case F_PAGED_JOIN: return run_body<F_PAGED_JOIN>(t, vb, smem, flag, EnterAlways());
+            case F_BEAM_SCAN: return run_body<F_BEAM_SCAN>(t, vb, smem, flag, EnterAlways());
+            case F_BEAM_PICK: return run_body<F_BEAM_PICK>(t, vb, smem, flag, EnterAlways());
+            default: break;
+        }
+    }
+    return true;
 }
 
 extern __shared__ __align__(16) unsigned char reef_dyn_smem[];
@@ -907,6 +914,10 @@ __global__ void __launch_bounds__(max_threads(F), min_blocks(F)) k_be(const __gr
 // resident on, not from its index: the reference assumes round-robin block placement over CUs
 // (reference: resource/mocked_kernel/mocked_kernel.trans.cu:112-186, blockIdx.x % 60), which
 // CUDA does not promise; tickets make the result independent of placement.
+// Two instances, by whether one of the two kernels belongs to a decoding step: the bodies of those take a stack frame of 704
+// bytes, 48 without them, and in one instance they slowed down the others (dispatcher flavour, us: vgg16 351, 330 without
+// them, BERT-base 698 and 682, DenseNet-201 1655 and 1625).
+static bool of_decoding_step(const KTask& t) { return t.family >= F_PAGE_TABLES && t.family <= F_BEAM_PICK; }
 __device__ __forceinline__ int next_ticket(int* counter, int* s_slot) {
     __syncthreads();
     if (threadIdx.x == 0) *s_slot = atomicAdd(counter, 1);
@@ -914,6 +925,7 @@ __device__ __forceinline__ int next_ticket(int* counter, int* s_slot) {
     return *s_slot;
 }
 
+template <bool DECODING>
 __global__ void __launch_bounds__(kThreads, 2) k_dispatch(const __grid_constant__ KTask rt, const __grid_constant__ KTask be,
                                                        int be_off, int be_num, int sm_partition,
                                                        int* __restrict__ be_slot, int* __restrict__ ctrl) {
@@ -929,13 +941,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_dispatch(const __grid_constant_
             for (;;) {
                 int v = next_ticket(&ctrl[0], &s_ticket);
                 if (v >= rt.nblocks) break;
-                run_any(rt, v, reef_dyn_smem, nullptr);
+                run_any<DECODING>(rt, v, reef_dyn_smem, nullptr);
             }
         } else {
             for (;;) {
                 int v = next_ticket(&ctrl[1], &s_ticket);
                 if (v >= be_num) break;
-                run_any(be, be_off + v, reef_dyn_smem, nullptr);
+                run_any<DECODING>(be, be_off + v, reef_dyn_smem, nullptr);
                 __syncthreads();
                 if (threadIdx.x == 0) red_release_gpu_add(be_slot, 1);
             }
@@ -1034,6 +1046,9 @@ int launch_delay(cudaStream_t st, unsigned long long ns) {
 // ------------------------------------------------------------------------------------------
 // host launchers
 // ------------------------------------------------------------------------------------------
+static const void* dispatch_fn(const KTask& rt, const KTask& be) {
+    return of_decoding_step(rt) || of_decoding_step(be) ? (const void*)k_dispatch<true> : (const void*)k_dispatch<false>;
+}
 unsigned long long launch_count() { return g_launches.load(std::memory_order_relaxed); }
 unsigned long long thread_launch_count() { return t_launches; }
 void add_launches(unsigned long long n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
@@ -1072,7 +1087,8 @@ static void prepare_carveout() {
         cudaFuncSetAttribute(plain_fn(f), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         cudaFuncSetAttribute(be_fn(f), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     }
-    cudaFuncSetAttribute((const void*)k_dispatch, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    for (const void* fn : {(const void*)k_dispatch<false>, (const void*)k_dispatch<true>})
+        cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     cudaFuncSetAttribute(plain_fn(F_ATTENTION_STAGED), cudaFuncAttributeMaxDynamicSharedMemorySize, att_smem(true));
     cudaFuncSetAttribute(be_fn(F_ATTENTION_STAGED), cudaFuncAttributeMaxDynamicSharedMemorySize, att_smem(true));
     // the GEMV's and the fp32 convolution's rings take more than the 48 KB a kernel gets without asking (also when the
@@ -1084,7 +1100,9 @@ static void prepare_carveout() {
     cudaFuncSetAttribute(plain_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesSmemMax);
     cudaFuncSetAttribute(be_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesSmemMax);
     paged_prepare_device();
-    cudaFuncSetAttribute((const void*)k_dispatch, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaFuncSetAttribute((const void*)k_dispatch<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         std::max(att_smem(true), std::max(kDenseSmem, kConvSimtSmem)));
+    cudaFuncSetAttribute((const void*)k_dispatch<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          std::max(std::max(att_smem(true), kTablesSmemMax), std::max(kDenseSmem, kConvSimtSmem)));
     int* w = nullptr;
     tc_error_word(&w);   // the device error word exists before any launch can be part of a stream capture
@@ -1272,7 +1290,7 @@ int launch_dispatch(const KernelSpec* rt, void** rt_args, const KernelSpec* be, 
         }
         int grid = num_sms * occupancy;
         void* kargs[] = {&trt, &tbe, &be_off, &be_num, &sm_partition, (void*)&be_slot, (void*)&ctrl};
-        cudaError_t e = cudaLaunchKernel((const void*)k_dispatch, dim3(grid), dim3(kThreads), kargs, smem, st);
+        cudaError_t e = cudaLaunchKernel(dispatch_fn(trt, tbe), dim3(grid), dim3(kThreads), kargs, smem, st);
         count_launch();
         return check_cuda(e, "cudaLaunchKernel(dispatch)");
     }
@@ -1291,7 +1309,7 @@ int launch_dispatch(const KernelSpec* rt, void** rt_args, const KernelSpec* be, 
             int grid = num_sms * occupancy;
             if (grid > trt.nblocks) grid = trt.nblocks;
             void* kargs[] = {&trt, &tbe, &zero, &zero, &part, (void*)&null_slot, (void*)&ctrl};
-            cudaError_t e = cudaLaunchKernel((const void*)k_dispatch, dim3(grid), dim3(kThreads), kargs, hosted_smem(*rt), st);
+            cudaError_t e = cudaLaunchKernel(dispatch_fn(trt, tbe), dim3(grid), dim3(kThreads), kargs, hosted_smem(*rt), st);
             count_launch();
             rc = check_cuda(e, "cudaLaunchKernel(dispatch rt)");
         }
@@ -1320,7 +1338,7 @@ int launch_dispatch(const KernelSpec* rt, void** rt_args, const KernelSpec* be, 
             return REEF_FAIL;
         }
         void* kargs[] = {&trt, &tbe, &be_off, &be_num, &part, (void*)&be_slot, (void*)&ctrl2};
-        cudaError_t e = cudaLaunchKernel((const void*)k_dispatch, dim3(grid), dim3(kThreads), kargs, hosted_smem(*be), bs);
+        cudaError_t e = cudaLaunchKernel(dispatch_fn(trt, tbe), dim3(grid), dim3(kThreads), kargs, hosted_smem(*be), bs);
         count_launch();
         return check_cuda(e, "cudaLaunchKernel(dispatch be)");
     }
@@ -1390,7 +1408,7 @@ int launch_dispatch_static(const KernelSpec* rt, void** rt_args, const KernelSpe
     if (occupancy < 1) occupancy = 1;
     int grid = num_sms * occupancy;
     void* kargs[] = {&trt, &tbe, &be_off, &be_num, &sm_partition, (void*)&be_slot, (void*)&ctrl};
-    cudaError_t e = cudaLaunchKernel((const void*)k_dispatch, dim3(grid), dim3(kThreads), kargs, smem, st);
+    cudaError_t e = cudaLaunchKernel(dispatch_fn(trt, tbe), dim3(grid), dim3(kThreads), kargs, smem, st);
     count_launch();
     return check_cuda(e, "cudaLaunchKernel(dispatch, static lane)");
 }
@@ -1433,7 +1451,8 @@ int kernel_attrs(const KernelSpec& s, reef_kernel_attrs_t* out) {
 }
 
 int dispatch_occupancy(uint32_t smem, int* occ) {
-    return check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(occ, (const void*)k_dispatch, kThreads, smem),
+    // (the same for either instance: two blocks of 128 registers to an SM; this one is allowed the most shared memory)
+    return check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(occ, (const void*)k_dispatch<true>, kThreads, smem),
                       "cudaOccupancyMaxActiveBlocksPerMultiprocessor(dispatch)");
 }
 
