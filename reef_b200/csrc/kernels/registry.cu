@@ -379,7 +379,7 @@ static int build_spec(const std::string& name, KernelSpec* s) {
         if (!a.need("s", &sN) || !a.need("h", &h) || !a.need("vocab", &vocab) || (h & 3)) goto bad;
         t.p.raw[0] = sN; t.p.raw[1] = h; t.p.raw[2] = vocab;
         if (!maybe_between(a, "npos", 1, 1 << 24, 0, &t.p.raw[3])) goto bad;
-        t.family = F_EMBEDDING;
+        t.family = t.p.raw[3] ? F_EMBEDDING_ROWS : F_EMBEDDING;
         t.nblocks = ceil_div(sN * (h / 4), kThreads * 4);
         s->nargs = t.p.raw[3] ? 5 : 4;
         s->bytes = 4.0 * 3.0 * sN * h + 8.0 * sN;
@@ -614,7 +614,8 @@ static void fill_arg_bytes(KernelSpec* s) {
         case F_SOFTMAX:
             b[0] = b[1] = f4((double)t.p.softmax.rows * t.p.softmax.n);
             break;
-        case F_EMBEDDING: {
+        case F_EMBEDDING:
+        case F_EMBEDDING_ROWS: {
             const double sN = t.p.raw[0], h = t.p.raw[1], vocab = t.p.raw[2];
             b[0] = f4(sN * h); b[1] = f4(vocab * h); b[2] = (size_t)sN * 8; b[3] = f4((t.p.raw[3] ? (double)t.p.raw[3] : sN) * h);
             if (t.p.raw[3]) b[4] = f4(4.0 * sN);
@@ -809,10 +810,11 @@ __device__ __forceinline__ bool run_body(const KTask& t, int vb, unsigned char* 
     if (F == F_COPY) return body_copy(t, vb, smem, flag);
     if (F == F_DENSE) return body_dense(t, vb, smem, flag);
     if (F == F_SOFTMAX) return body_softmax(t, vb, smem, flag);
-    if (F == F_EMBEDDING) return body_embedding(t, vb, smem, flag);
+    if (F == F_EMBEDDING) return body_embedding<false>(t, vb, smem, flag);
     if (F == F_LAYERNORM) return body_layernorm(t, vb, smem, flag);
     if (F == F_ATTENTION) return attention_rows<false>(t, vb, smem, flag);
     if (F == F_ATTENTION_STAGED) return attention_rows<true>(t, vb, smem, flag);
+    if (F == F_EMBEDDING_ROWS) return body_embedding<true>(t, vb, smem, flag);
     if (F == F_PAGE_TABLES) return body_page_tables(t, vb, smem, flag);
     if (F == F_PAGED_APPEND) return body_paged_append(t, vb, smem, flag);
     if (F == F_PAGED_JOIN) return body_paged_join(t, vb, smem, flag);
@@ -846,6 +848,7 @@ __device__ __noinline__ bool run_any(const KTask& t, int vb, unsigned char* smem
     }
     if (DECODING) {
         switch (t.family) {
+            case F_EMBEDDING_ROWS: return run_body<F_EMBEDDING_ROWS>(t, vb, smem, flag, EnterAlways());
             case F_PAGE_TABLES: return run_body<F_PAGE_TABLES>(t, vb, smem, flag, EnterAlways());
             case F_PAGED_APPEND: return run_body<F_PAGED_APPEND>(t, vb, smem, flag, EnterAlways());
             case F_PAGED_JOIN: return run_body<F_PAGED_JOIN>(t, vb, smem, flag, EnterAlways());
@@ -915,9 +918,9 @@ __global__ void __launch_bounds__(max_threads(F), min_blocks(F)) k_be(const __gr
 // (reference: resource/mocked_kernel/mocked_kernel.trans.cu:112-186, blockIdx.x % 60), which
 // CUDA does not promise; tickets make the result independent of placement.
 // Two instances, by whether one of the two kernels belongs to a decoding step: the bodies of those take a stack frame of 704
-// bytes, 48 without them, and in one instance they slowed down the others (dispatcher flavour, us: vgg16 351, 330 without
-// them, BERT-base 698 and 682, DenseNet-201 1655 and 1625).
-static bool of_decoding_step(const KTask& t) { return t.family >= F_PAGE_TABLES && t.family <= F_BEAM_PICK; }
+// bytes, 48 without them, and in one instance they slowed down the others (dispatcher flavour, us: vgg16 351, 333 without
+// them, BERT-base 698 and 689, DenseNet-201 1655 and 1608).
+static bool of_decoding_step(const KTask& t) { return t.family >= F_EMBEDDING_ROWS && t.family <= F_BEAM_PICK; }
 __device__ __forceinline__ int next_ticket(int* counter, int* s_slot) {
     __syncthreads();
     if (threadIdx.x == 0) *s_slot = atomicAdd(counter, 1);
@@ -1056,7 +1059,7 @@ void add_launches(unsigned long long n) { g_launches.fetch_add(n, std::memory_or
 #define FOR_EACH_FAMILY(X)                                                                      \
     X(F_MOCK_ADD) X(F_MOCK_MUL) X(F_FUSED_ADD_NCHW) X(F_BIAS_RELU) X(F_CONV_SIMT) X(F_MAX_POOL) \
     X(F_AVG_POOL) X(F_GLOBAL_AVG_POOL) X(F_COPY) X(F_DENSE) X(F_SOFTMAX) X(F_EMBEDDING) X(F_LAYERNORM) X(F_ATTENTION) X(F_ATTENTION_STAGED) \
-    X(F_NCHW_TO_NHWC4) X(F_IM2COL_NCHW) X(F_PAGE_TABLES) X(F_PAGED_APPEND) X(F_PAGED_JOIN) X(F_BEAM_SCAN) X(F_BEAM_PICK)
+    X(F_NCHW_TO_NHWC4) X(F_IM2COL_NCHW) X(F_EMBEDDING_ROWS) X(F_PAGE_TABLES) X(F_PAGED_APPEND) X(F_PAGED_JOIN) X(F_BEAM_SCAN) X(F_BEAM_PICK)
 
 static const void* plain_fn(int family) {
     switch (family) {

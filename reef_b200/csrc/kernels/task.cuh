@@ -35,6 +35,7 @@ enum Family : int {
     F_ATTENTION_STAGED,
     F_NCHW_TO_NHWC4,
     F_IM2COL_NCHW,
+    F_EMBEDDING_ROWS,   // the first of a decoding step's, F_BEAM_PICK the last
     F_PAGE_TABLES,
     F_PAGED_APPEND,
     F_PAGED_JOIN,
