@@ -72,11 +72,8 @@ static const void* paged_fn(const PagedP& p) {
     return p.kt == KT_FP32 ? paged_fn_dim<float>(p.d, p.gb) : p.kt == KT_BF16 ? paged_fn_dim<__nv_bfloat16>(p.d, p.gb) : paged_fn_dim<__half>(p.d, p.gb);
 }
 
-// once per device, ahead of the first launch (reef_kernel_prepare)
+// on the current device, ahead of the first launch there: a part of what reef_kernel_prepare does once
 int paged_prepare_device() {
-    static bool done[16] = {false};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16 || done[dev]) return REEF_SUCC;
     for (int kt = KT_FP32; kt <= KT_FP16; kt++)
         for (int d = 64; d <= 256; d *= 2)
             for (int gb = 1; gb <= 8; gb++) {
@@ -91,7 +88,6 @@ int paged_prepare_device() {
                     return REEF_FAIL;
                 }
             }
-    done[dev] = true;
     return REEF_SUCC;
 }
 

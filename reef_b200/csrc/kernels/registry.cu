@@ -1083,34 +1083,48 @@ static const void* be_fn(int family) {
 // SM: behind a tensor-core kernel that fills every SM, a kernel with another preference had to wait for whole
 // SMs to drain and be reconfigured (BERT-base replay 0.92 -> 1.13 ms with 216-CTA matmul plans).
 static bool g_carveout_set[16] = {false};
-static void prepare_carveout() {
+static int check_cuda(cudaError_t e, const char* what);
+static int prepare_carveout() {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16 || g_carveout_set[dev]) return;
-    for (int f = 0; f < F_COUNT; f++) {
-        cudaFuncSetAttribute(plain_fn(f), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        cudaFuncSetAttribute(be_fn(f), cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return check_cuda(e, "cudaGetDevice(prepare)");
+    if (dev < 0 || dev >= 16) {
+        set_error("device " + std::to_string(dev) + ": kernels are prepared on devices 0 to 15");
+        return REEF_OUT_OF_RANGE;
     }
-    for (const void* fn : {(const void*)k_dispatch<false>, (const void*)k_dispatch<true>})
-        cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    cudaFuncSetAttribute(plain_fn(F_ATTENTION_STAGED), cudaFuncAttributeMaxDynamicSharedMemorySize, att_smem(true));
-    cudaFuncSetAttribute(be_fn(F_ATTENTION_STAGED), cudaFuncAttributeMaxDynamicSharedMemorySize, att_smem(true));
+    if (g_carveout_set[dev]) return REEF_SUCC;
+    // the first error of all; a device is prepared when there was none, else the next call tries again
+    auto set = [&](const void* fn, cudaFuncAttribute what, int value) {
+        const cudaError_t now = cudaFuncSetAttribute(fn, what, value);
+        if (e == cudaSuccess) e = now;
+    };
+    auto carve = [&](const void* fn) { set(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); };
+    auto most = [&](const void* fn, int bytes) { set(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
+    for (int f = 0; f < F_COUNT; f++) {
+        carve(plain_fn(f));
+        carve(be_fn(f));
+    }
+    carve((const void*)k_dispatch<false>);
+    carve((const void*)k_dispatch<true>);
+    most(plain_fn(F_ATTENTION_STAGED), att_smem(true));
+    most(be_fn(F_ATTENTION_STAGED), att_smem(true));
     // the GEMV's and the fp32 convolution's rings take more than the 48 KB a kernel gets without asking (also when the
     // dispatcher hosts them)
-    cudaFuncSetAttribute(plain_fn(F_CONV_SIMT), cudaFuncAttributeMaxDynamicSharedMemorySize, kConvSimtSmem);
-    cudaFuncSetAttribute(be_fn(F_CONV_SIMT), cudaFuncAttributeMaxDynamicSharedMemorySize, kConvSimtSmem);
-    cudaFuncSetAttribute(plain_fn(F_DENSE), cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
-    cudaFuncSetAttribute(be_fn(F_DENSE), cudaFuncAttributeMaxDynamicSharedMemorySize, kDenseSmem);
-    cudaFuncSetAttribute(plain_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesSmemMax);
-    cudaFuncSetAttribute(be_fn(F_PAGE_TABLES), cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesSmemMax);
-    paged_prepare_device();
-    cudaFuncSetAttribute((const void*)k_dispatch<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         std::max(att_smem(true), std::max(kDenseSmem, kConvSimtSmem)));
-    cudaFuncSetAttribute((const void*)k_dispatch<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         std::max(std::max(att_smem(true), kTablesSmemMax), std::max(kDenseSmem, kConvSimtSmem)));
+    most(plain_fn(F_CONV_SIMT), kConvSimtSmem);
+    most(be_fn(F_CONV_SIMT), kConvSimtSmem);
+    most(plain_fn(F_DENSE), kDenseSmem);
+    most(be_fn(F_DENSE), kDenseSmem);
+    most(plain_fn(F_PAGE_TABLES), kTablesSmemMax);
+    most(be_fn(F_PAGE_TABLES), kTablesSmemMax);
+    most((const void*)k_dispatch<false>, std::max(att_smem(true), std::max(kDenseSmem, kConvSimtSmem)));
+    most((const void*)k_dispatch<true>, std::max(std::max(att_smem(true), kTablesSmemMax), std::max(kDenseSmem, kConvSimtSmem)));
+    int rc = check_cuda(e, "cudaFuncSetAttribute(prepare)");
+    if (rc == REEF_SUCC) rc = paged_prepare_device();
     int* w = nullptr;
-    tc_error_word(&w);   // the device error word exists before any launch can be part of a stream capture
+    if (rc == REEF_SUCC) rc = tc_error_word(&w);   // the device error word exists before any launch can be part of a stream capture
     cudaGetLastError();
-    g_carveout_set[dev] = true;
+    g_carveout_set[dev] = rc == REEF_SUCC;
+    return rc;
 }
 
 // Launch with the programmatic-stream-serialization attribute: the kernel may be scheduled while its predecessor
@@ -1199,8 +1213,8 @@ int make_chain(const KernelSpec* const* specs, void*** args, int n, int clusters
 }
 
 int prepare_kernel(const KernelSpec& s, void** args) {
-    prepare_carveout();
-    if (s.task.family == F_PAGED_ATTENTION) return paged_prepare_device();
+    const int rc = prepare_carveout();
+    if (rc != REEF_SUCC || s.task.family == F_PAGED_ATTENTION) return rc;
     if (is_own_family(s.task.family)) return bind_tc(s, args);
     return REEF_SUCC;
 }

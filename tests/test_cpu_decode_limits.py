@@ -1,0 +1,25 @@
+"""What the decoding operators report and refuse, where no GPU is needed to see it."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+pytestmark = pytest.mark.usefixtures("libs")
+
+
+def _run(code, **env):
+    """A process of its own that sees no GPU."""
+    return subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**os.environ, "CUDA_VISIBLE_DEVICES": "", **env}, capture_output=True, text=True,
+                          timeout=300)
+
+
+@pytest.mark.parametrize("name", ["reef_page_tables__rows16_mp64_ps16_pages1024_tokens16", "reef_paged_append__tokens16_kvh12_d64_ps16_pages1024_kt1",
+                                  "reef_paged_attention__tokens16_rows16_heads12_kvh12_d64_ps16_mp64_pages1024_kt0",
+                                  "reef_beam_scan__requests4_beams4_vocab1000", "add"])
+def test_a_device_that_cannot_be_prepared_is_reported(name):
+    """A kernel whose setup has failed must not look ready: its launches would fail later, with another message."""
+    r = _run(f"from reef_b200 import capi\nk = capi.Kernel({name!r})\ntry:\n    k.prepare([0] * k.num_args)\nexcept capi.ReefError as e:\n"
+             "    print('status', e.status, 'no CUDA' in str(e) or 'driver' in str(e))")
+    assert r.stdout.strip() == "status 1 True", r.stdout + r.stderr
