@@ -26,9 +26,17 @@ import torch
 from .capi import FAIL, OUT_OF_RANGE, Kernel, ReefError, cuda_lib
 from .resources import decoding
 
-cuda_lib()                      # (raises where the libraries are not built)
-from . import _decode           # noqa: E402
 
+class _Unbuilt:
+    """Stands for the native module until the first call: the libraries need not be built to import this one."""
+    def __getattr__(self, name):
+        global _decode
+        cuda_lib()              # (raises where the libraries are not built)
+        from . import _decode
+        return getattr(_decode, name)
+
+
+_decode = _Unbuilt()
 _TYPES = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16"}
 
 

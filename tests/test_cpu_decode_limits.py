@@ -1,5 +1,6 @@
 """What the decoding operators report and refuse, where no GPU is needed to see it."""
 import os
+import shutil
 import subprocess
 import sys
 
@@ -23,3 +24,12 @@ def test_a_device_that_cannot_be_prepared_is_reported(name):
     r = _run(f"from reef_b200 import capi\nk = capi.Kernel({name!r})\ntry:\n    k.prepare([0] * k.num_args)\nexcept capi.ReefError as e:\n"
              "    print('status', e.status, 'no CUDA' in str(e) or 'driver' in str(e))")
     assert r.stdout.strip() == "status 1 True", r.stdout + r.stderr
+
+
+def test_the_module_can_be_imported_before_the_libraries_are_built(tmp_path):
+    """A clone that is not built: tests are collected, and a call says what is missing."""
+    shutil.copytree(os.path.join(ROOT, "reef_b200"), tmp_path / "reef_b200", ignore=shutil.ignore_patterns("*.so", "csrc", "__pycache__"))
+    r = subprocess.run([sys.executable, "-c", "import torch\nfrom reef_b200 import capi, decode\nx = torch.zeros(2, 4, dtype=torch.int32)\n"
+                        "try:\n    decode.page_tables(x, x[0], x[1], pages=1, page_size=1, tokens=1)\nexcept capi.ReefError as e:\n    print(e)"],
+                       cwd=tmp_path, capture_output=True, text=True, timeout=300)
+    assert "is not built" in r.stdout, r.stdout + r.stderr
