@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import glob
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -111,8 +112,12 @@ def build_torch(verbose: bool = False) -> str:
 
 
 def build_all(verbose: bool = False):
+    """Both libraries, and where torch is installed its module too: nothing else here needs torch."""
     cuda, host = build_cuda(verbose), build_host(verbose)
-    build_torch(verbose)
+    if importlib.util.find_spec("torch") is not None:
+        build_torch(verbose)
+    elif verbose:
+        print("[reef_b200.build] torch is not installed: without decode.py's calls on its tensors")
     return cuda, host
 
 

@@ -33,3 +33,8 @@ def test_the_module_can_be_imported_before_the_libraries_are_built(tmp_path):
                         "try:\n    decode.page_tables(x, x[0], x[1], pages=1, page_size=1, tokens=1)\nexcept capi.ReefError as e:\n    print(e)"],
                        cwd=tmp_path, capture_output=True, text=True, timeout=300)
     assert "is not built" in r.stdout, r.stdout + r.stderr
+
+
+def test_the_libraries_are_built_without_torch():
+    r = _run("import sys\nsys.modules['torch'] = None\nfrom reef_b200 import build, capi\nprint(len(build.build_all()))\ncapi.kernel_plan('add')")
+    assert r.stdout.strip() == "2" and r.returncode == 0, r.stdout + r.stderr
