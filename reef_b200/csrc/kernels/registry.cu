@@ -177,7 +177,7 @@ static bool build_paged(const std::string& op, const Attrs& a, KernelSpec* s) {
     if ((long long)p.pages * p.ps * p.kvh > 0x7fffffffLL) return false;   // a key's place is an int
     const long long passes = (long long)p.tokens * p.kvh * p.subs;
     const int units = ceil_div(p.mp * p.ps, paged_unit(p));
-    if (passes * units > 0x70000000LL) return false;
+    if ((parts || join) && passes * units > 0x70000000LL) return false;   // (only there all rows' units are added up, in an int)
     const int blocks = paged_parts_blocks(p, passes * units);
     if (join) {
         p.split = blocks;

@@ -114,6 +114,13 @@ def _whole(what, name, v, lo, hi):
         _refuse(what, f"{name} = {v!r} is not a whole number from {lo} to {hi}")
 
 
+def _at_most(what, **limits):
+    """What the kernels' whole numbers hold: name=(value, limit)."""
+    for name, (v, most) in limits.items():
+        if v > most:
+            _refuse(what, f"{name.replace('_', ' ')}: {v}, at most {most}")
+
+
 def _token_stride(what, name, t, heads, dim):
     """[tokens][heads][dim] with any stride from token to token that keeps 16-byte loads aligned."""
     if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != dim and heads > 1:
@@ -185,6 +192,7 @@ def _page_tables(what, why, inputs, outputs, options):
         _whole(what, name, v, 1, hi)
     if not 1 <= rows <= 1024 or max_pages < 1:
         _refuse(what, f"a table of {tuple(table.shape)}: 1 to 1024 rows of a page or more")
+    _at_most(what, tokens_of_a_row=(max_pages * page_size, 1 << 30), ids_of_the_table=(rows * max_pages, 1 << 30))
     _want(what, "table", table, table.shape)
     _want(what, "lens", lens, (rows,), device=device)
     _want(what, "new", new, (rows,), device=device)
@@ -207,9 +215,10 @@ def _page_tables(what, why, inputs, outputs, options):
 def _cache(what, k_cache, v_cache, device):
     if k_cache.dim() != 4 or k_cache.dtype not in _TYPES:
         _refuse(what, f"k_cache is {k_cache.dtype} {tuple(k_cache.shape)}, not fp32, bf16 or fp16 [pages][kv heads][page size][dim]")
+    pages, kv, page, dim = k_cache.shape
+    _at_most(what, kv_heads=(kv, 1024), tokens_of_a_page=(page, 1024), tokens_of_the_cache=(pages * page, 0x7fffffff))
     _want(what, "k_cache", k_cache, k_cache.shape, k_cache.dtype, device)
     _want(what, "v_cache", v_cache, k_cache.shape, k_cache.dtype, device)
-    pages, kv, page, dim = k_cache.shape
     if dim not in (64, 128, 256):
         _refuse(what, f"heads of {dim} dimensions: 64, 128 or 256")
     return pages, kv, page, dim
@@ -236,6 +245,12 @@ def _paged_append(what, why, inputs):
     _tensors(what, k=k, v=v, tok=tok, k_cache=k_cache, v_cache=v_cache)
     _inference(what, *inputs)
     device = k.device
+    if k.dim() == 3:
+        _at_most(what, tokens=(k.shape[0], 1 << 20), values_of_all_tokens=(k.shape.numel(), 0x70000000))
+    if fork is not None:
+        if not isinstance(fork, torch.Tensor) or fork.dim() != 2 or not fork.shape[0]:
+            _refuse(what, "fork is not [rows][4]")
+        _at_most(what, forks=(fork.shape[0], 1 << 20))
     pages, kv, page, dim = _cache(what, k_cache, v_cache, device)
     shape = (k.shape[0] if k.dim() else 0, kv, dim)
     _want(what, "k", k, shape, torch.float32, device, dense=False)
@@ -244,8 +259,6 @@ def _paged_append(what, why, inputs):
     if not shape[0]:
         _refuse(what, "no tokens")
     if fork is not None:
-        if not isinstance(fork, torch.Tensor) or fork.dim() != 2 or not fork.shape[0]:
-            _refuse(what, "fork is not [rows][4]")
         _want(what, "fork", fork, (fork.shape[0], 4), device=device)
     strides = dict(ks=_token_stride(what, "k", k, kv, dim), vs=_token_stride(what, "v", v, kv, dim))
     kernels = _resolve(what, device, [decoding.paged_append(shape[0], kv, dim, page, pages, _TYPES[k_cache.dtype],
@@ -264,6 +277,8 @@ def paged_attention(q, k_cache, v_cache, table, tok, *, out=None):
     of its row, but for those on pages whose id is outside the cache; where it sees none (a token without a row, length 0) its
     output is zero.  Scores are scaled by 1 / sqrt(dim); sums and the softmax are fp32 whatever the cache's type.  Returns
     [tokens][heads][dim] fp32.
+
+    Up to 65536 tokens and rows, 1024 heads, pages of 1024 tokens, rows of 2^30; pages * kv heads * page size of the cache are below 2^31.
     """
     inputs, outputs = (q, k_cache, v_cache, table, tok), None if out is None else (out,)
     got = _decode.call(_ATTENTION, inputs, outputs, ())
@@ -279,6 +294,9 @@ def _paged_attention(what, why, inputs, outputs):
     _tensors(what, q=q, k_cache=k_cache, v_cache=v_cache, table=table, tok=tok)
     _inference(what, *inputs)
     device = q.device
+    if q.dim() == 3 and table.dim() == 2 and k_cache.dim() == 4:
+        _at_most(what, tokens=(q.shape[0], 1 << 16), heads=(q.shape[1], 1024), rows=(table.shape[0], 1 << 16),
+                 tokens_of_a_row=(table.shape[1] * k_cache.shape[2], 1 << 30), keys_of_the_cache=(k_cache.shape[:3].numel(), 0x7fffffff))
     pages, kv, page, dim = _cache(what, k_cache, v_cache, device)
     if q.dim() != 3 or not q.shape[0] or not q.shape[1] or q.shape[1] % kv:
         _refuse(what, f"q of {tuple(q.shape)}: [tokens][heads][dim], heads a multiple of {kv}")
@@ -330,6 +348,7 @@ def _beam_select(what, why, inputs, outputs, options):
     _whole(what, "beams", beams, 1, 16)
     _whole(what, "eos", eos, 0, logits.shape[1] - 1)
     rows = score.shape[0] if score.dim() else 0
+    _at_most(what, words=(logits.shape[1], 0x7fffffff // 16), rows=(rows, 1 << 20), rows_of_logits=(logits.shape[0], 1 << 20))
     if not rows or rows % beams or (start is None and logits.shape[0] != rows):
         _refuse(what, f"{rows} scores, {logits.shape[0]} rows of logits, {beams} beams to a request")
     _want(what, "logits", logits, logits.shape, torch.float32, device)

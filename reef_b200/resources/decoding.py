@@ -31,12 +31,20 @@ def paged_attention(tokens: int, rows: int, heads: int, kv_heads: int, dim: int,
     a head are B bytes): 12 heads of all rows, B = 512 KB 14.5 / 13.4 for the longest and 6.3 / 12.5 for a short one; 64, 1 MB 22.7 / 20.8 (6);
     192, 512 KB 18.6 / 20 (11), 1 MB 30.8 / 33.7 (18), 2 MB 54 / 53 (38); 512, 1 MB 71 / 70 (46); 768, 1 MB 79 / 88 (69), 2 MB 153 / 155 (139); 2048,
     1 MB 185 / 207 (164); but 512 of very uneven rows, 4 MB, would wait for the longest.  One kernel, therefore, up to 512 KB and as much
-    again for every 320 heads."""
+    again for every 320 heads; and where the steps of all rows are more than the division among blocks counts (0x70000000)."""
     shape = dict(tokens=tokens, rows=rows, heads=heads, kvh=kv_heads, d=dim, ps=page_size, mp=max_pages, pages=pages, kt=CACHE_TYPES[cache])
     longest = 2 * max_pages * page_size * dim * (4 if cache == "float32" else 2)
+    one = [kname("reef_paged_attention", **shape, **strides)]
     if longest <= (512 << 10) * (1 + tokens * kv_heads / 320):
-        return [kname("reef_paged_attention", **shape, **strides)]
-    return [kname("reef_paged_attention_parts", **shape, **strides), kname("reef_paged_attention_join", **shape)]
+        return one
+    two = [kname("reef_paged_attention_parts", **shape, **strides), kname("reef_paged_attention_join", **shape)]
+    if tokens * heads * max_pages * page_size >= 0x70000000:        # (a step takes a key at least)
+        from .. import capi
+        try:
+            capi.kernel_plan(two[0])
+        except capi.ReefError:
+            return one
+    return two
 
 
 def beam_select(requests: int, beams: int, vocab: int, eos: int, tokens: int | None = None) -> list:

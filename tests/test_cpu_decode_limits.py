@@ -5,6 +5,10 @@ import subprocess
 import sys
 
 import pytest
+import torch
+
+from reef_b200 import capi, decode
+from reef_b200.resources import decoding
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.usefixtures("libs")
@@ -38,3 +42,79 @@ def test_the_module_can_be_imported_before_the_libraries_are_built(tmp_path):
 def test_the_libraries_are_built_without_torch():
     r = _run("import sys\nsys.modules['torch'] = None\nfrom reef_b200 import build, capi\nprint(len(build.build_all()))\ncapi.kernel_plan('add')")
     assert r.stdout.strip() == "2" and r.returncode == 0, r.stdout + r.stderr
+
+
+# the steps of all rows together (0x70000000) bound the form that adds them up, not the one that takes a row to a block
+WIDE = dict(heads=32, kv_heads=32, dim=128, page_size=64, max_pages=2048, pages=4096, cache="bfloat16")
+
+
+def test_many_tokens_over_long_tables():
+    for tokens, fits in ((3583, True), (8192, False)):          # 32 passes a token, 16384 steps a pass
+        names = decoding.paged_attention(tokens, 4, **WIDE)
+        assert len(names) == 1
+        capi.kernel_plan(names[0])
+        for form in ("parts", "join"):
+            name = names[0].replace("attention__", f"attention_{form}__")
+            if fits:
+                capi.kernel_plan(name)
+            else:
+                with pytest.raises(capi.ReefError):
+                    capi.kernel_plan(name)
+    # tables so long that the division among blocks would be taken: only as far as it can count
+    for tokens, forms in ((64, 2), (4096, 2), (8192, 1)):
+        names = decoding.paged_attention(tokens, 4, 1, 1, 256, 1024, 512, 600, "float32")
+        assert len(names) == forms
+        for name in names:
+            capi.kernel_plan(name)
+
+
+def _big(*shape, dtype=torch.int32):
+    return torch.zeros(1, dtype=dtype).expand(*shape)
+
+
+def _why(fn, *args, **kw):
+    with pytest.raises(capi.ReefError) as e:
+        fn(*args, **kw)
+    assert e.value.status == capi.OUT_OF_RANGE
+    return str(e.value)
+
+
+def test_sizes_beyond_the_kernels_are_named():
+    f = torch.float32
+
+    def attend(tokens=2, heads=2, rows=2, most=4, pages=8, kv=1, page=16):
+        c = _big(pages, kv, page, 64, dtype=f)
+        return _why(decode.paged_attention, _big(tokens, heads, 64, dtype=f), c, c, _big(rows, most), _big(tokens, 4))
+
+    assert "not on a GPU" in attend() and "not on a GPU" in attend(tokens=65536, rows=65536, heads=1024, page=1024, most=1 << 20)
+    assert "tokens: 65537, at most 65536" in attend(tokens=65537)
+    assert "rows: 65537, at most 65536" in attend(rows=65537)
+    assert "heads: 1025, at most 1024" in attend(heads=1025)
+    assert "tokens of a page: 1025, at most 1024" in attend(page=1025)
+    assert "tokens of a row: " in attend(most=(1 << 26) + 1)
+    assert "keys of the cache: " in attend(pages=1 << 23, kv=16)
+
+    def append(tokens=2, kv=1, forks=None, pages=8):
+        c, k = _big(pages, kv, 16, 64, dtype=f), _big(tokens, kv, 64, dtype=f)
+        return _why(decode.paged_append, k, k, _big(tokens, 4), c, c, fork=None if forks is None else _big(forks, 4))
+
+    assert "not on a GPU" in append() and "not on a GPU" in append(tokens=1 << 20, forks=1 << 20)
+    assert "tokens: 1048577, at most 1048576" in append(tokens=(1 << 20) + 1)
+    assert "values of all tokens: " in append(tokens=1 << 20, kv=32)
+    assert "forks: 1048577, at most 1048576" in append(forks=(1 << 20) + 1)
+    assert "kv heads: 1025, at most 1024" in append(kv=1025)
+    assert "tokens of the cache: " in append(pages=1 << 27)
+
+    def tables(rows=2, most=4, page=16):
+        return _why(decode.page_tables, _big(rows, most), _big(rows), _big(rows), pages=8, page_size=page, tokens=2)
+
+    assert "not on a GPU" in tables() and "not on a GPU" in tables(rows=1024, most=1 << 20)
+    assert "tokens of a row: " in tables(most=(1 << 26) + 1)
+    assert "ids of the table: " in tables(rows=1024, most=(1 << 20) + 1)
+
+    def beams(rows=2, words=100, start=None):
+        return _why(decode.beam_select, _big(rows, words, dtype=f), _big(rows, dtype=f), _big(rows), beams=1, eos=0)
+
+    assert "not on a GPU" in beams() and "not on a GPU" in beams(rows=1 << 20)
+    assert "words: " in beams(words=1 << 27)
+    assert "rows: 1048577" in beams(rows=(1 << 20) + 1)
