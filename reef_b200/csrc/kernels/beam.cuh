@@ -1,6 +1,6 @@
 // Beam search's selection: of every request the `beams` best continuations over its beams and the vocabulary,
 //   cand(b, w) = score[b] + logits[b][w] - log sum_u exp(logits[b][u]),
-// ties by the lowest b * vocab + w.  A beam that has ended (live 0) competes with its score and the end word alone; candidates of
+// ties by the lower beam, then the greater logit, then the lower word.  A beam that has ended (live 0) competes with its score and the end word alone; candidates of
 // -infinity or NaN are none, so a row without a finite sum (a NaN, an infinity, nothing but -infinity) has none, nor has a beam without a
 // finite score.  What is missing comes out as token -1, parent -1, score -infinity, live 0.
 #pragma once
@@ -22,25 +22,27 @@ __host__ inline int beam_parts(long long rows, int vocab) {
 }
 __host__ __device__ inline int beam_part_floats(int beams) { return 2 + 2 * beams; }
 
-template <class V>
+// V: values, I: what decides between equal ones, the lowest first
+template <class V, class I>
 struct BeamRoom {
     V value[kBeamRoom];
-    int index[kBeamRoom];
+    I index[kBeamRoom];
     V line[8];
-    int who[8];
+    I who[8];
     int count;
 };
-constexpr int kBeamSmem = (int)sizeof(BeamRoom<double>);
+typedef unsigned long long BeamKey;
+constexpr int kBeamSmem = (int)sizeof(BeamRoom<double, BeamKey>);
 
-template <class V>
-__device__ __forceinline__ bool beam_before(V a, int ia, V b, int ib) { return a > b || (a == b && ia < ib); }
+template <class V, class I>
+__device__ __forceinline__ bool beam_before(V a, I ia, V b, I ib) { return a > b || (a == b && ia < ib); }
 
 // `each(f)` calls f(value, index) for the values of this thread; -infinity and NaN are none.  block_collect gathers those of all threads (s.count
 // is 0 before, the threads have not met behind it), block_place ranks them, if there is room for all, ties by the lowest index, and calls
 // `take(i, value, index)` for the i-th of the K greatest; both it and block_top return how many of these there are.
-template <class V, class Each>
-__device__ __forceinline__ void block_collect(BeamRoom<V>& s, Each each) {
-    each([&](V v, int i) {
+template <class V, class I, class Each>
+__device__ __forceinline__ void block_collect(BeamRoom<V, I>& s, Each each) {
+    each([&](V v, I i) {
         if (v > (V)-INFINITY) {
             const int at = atomicAdd(&s.count, 1);
             if (at < kBeamRoom) {
@@ -50,11 +52,11 @@ __device__ __forceinline__ void block_collect(BeamRoom<V>& s, Each each) {
         }
     });
 }
-template <class V, class Take>
-__device__ __forceinline__ int block_place(int K, const BeamRoom<V>& s, int n, Take take) {
+template <class V, class I, class Take>
+__device__ __forceinline__ int block_place(int K, const BeamRoom<V, I>& s, int n, Take take) {
     for (int c = threadIdx.x; c < n; c += kThreads) {
         const V v = s.value[c];
-        const int i = s.index[c];
+        const I i = s.index[c];
         int r = 0;
 #pragma unroll 4
         for (int o = 0; o < n; o++) r += beam_before(s.value[o], s.index[o], v, i);
@@ -64,8 +66,8 @@ __device__ __forceinline__ int block_place(int K, const BeamRoom<V>& s, int n, T
 }
 // Every warp's K-th greatest of its lanes' values has K values at or above it, so the greatest of these eight is a line that few values reach.
 // (s.count is 0 behind it.)
-template <class V>
-__device__ __forceinline__ V block_line(int K, BeamRoom<V>& s, V top) {
+template <class V, class I>
+__device__ __forceinline__ V block_line(int K, BeamRoom<V, I>& s, V top) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int rank = 0;
 #pragma unroll 4
@@ -83,29 +85,31 @@ __device__ __forceinline__ V block_line(int K, BeamRoom<V>& s, V top) {
     return line;
 }
 // The line is drawn through the threads' maxima.  Where more reach it than there is room for (many equal values) the best one behind the last is looked for K times.
-template <class V, class Each, class Take>
-__device__ __forceinline__ int block_top(int K, BeamRoom<V>& s, Each each, Take take) {
+template <class V, class I, class Each, class Take>
+__device__ __forceinline__ int block_top(int K, BeamRoom<V, I>& s, Each each, Take take) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const V ninf = -INFINITY;
     V top = ninf;
-    each([&](V v, int) { if (v > top) top = v; });
-    const V line = block_line<V>(K, s, top);
-    block_collect<V>(s, [&](auto f) { each([&](V v, int i) { if (v >= line) f(v, i); }); });
+    each([&](V v, I) { if (v > top) top = v; });
+    const V line = block_line(K, s, top);
+    block_collect(s, [&](auto f) { each([&](V v, I i) { if (v >= line) f(v, i); }); });
     __syncthreads();
     const int n = s.count;
-    if (n <= kBeamRoom) return block_place<V>(K, s, n, take);
+    if (n <= kBeamRoom) return block_place(K, s, n, take);
+    constexpr I none = sizeof(I) == 4 ? (I)0x7fffffff : ~(I)0;
     V last = INFINITY;
-    int last_i = -1, found = 0;
+    I last_i = (I)-1;               // (of the keys it is the highest, but their values are finite)
+    int found = 0;
     for (; found < K; found++) {
         V best = ninf;
-        int best_i = 0x7fffffff;
-        each([&](V v, int i) {
+        I best_i = none;
+        each([&](V v, I i) {
             if (v > ninf && beam_before(last, last_i, v, i) && beam_before(v, i, best, best_i)) best = v, best_i = i;
         });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const V v = __shfl_xor_sync(0xffffffffu, best, o);
-            const int i = __shfl_xor_sync(0xffffffffu, best_i, o);
+            const I i = __shfl_xor_sync(0xffffffffu, best_i, o);
             if (beam_before(v, i, best, best_i)) best = v, best_i = i;
         }
         __syncthreads();
@@ -140,7 +144,7 @@ __device__ __forceinline__ int beam_logits(const BeamP& p, const int* start, int
 // line, the second look and the ranking, during which little is read; four rows of 30522 words 6.  Code of many unrolled steps after the pass is itself slow, every line of
 // it being fetched once: a loop unrolled 16 times took 1 us longer than the loop.
 struct BeamScan {
-    BeamRoom<float> room;
+    BeamRoom<float, int> room;
     float key[8][32];            // of every warp and group the greatest word and the turn it came in
     int turn[8][32];
     float top[8], sum[8];
@@ -300,10 +304,10 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
         out[2 + i] = v;
         out[2 + K + i] = __int_as_float(w);
     };
-    block_collect<float>(s.room, each);
+    block_collect(s.room, each);
     __syncthreads();
     const int n = s.room.count;
-    const int found = n <= kBeamRoom ? block_place<float>(K, s.room, n, take) : block_top<float>(K, s.room, each, take);
+    const int found = n <= kBeamRoom ? block_place(K, s.room, n, take) : block_top(K, s.room, each, take);
     if (tid >= found && tid < K) {
         out[2 + tid] = -INFINITY;
         out[2 + K + tid] = __int_as_float(0);
@@ -312,8 +316,9 @@ __device__ __forceinline__ bool body_beam_scan(const KTask& t, int vb, unsigned 
 }
 
 // ---- pick: the parts of a request's beams -> its new beams --------------------------------------------------------------------
-// args: parts, score, live, [start], token, parent, score', live'.  Within a beam the logits decide, exactly as they are; beams are
-// compared in 64 bits: a score of -50 in 32 bits cannot tell logits apart that differ by less than 4e-6.  Latency: 32 requests of eight beams
+// args: parts, score, live, [start], token, parent, score', live'.  Beams are compared in 64 bits: a score of -50 in 32 bits cannot tell logits
+// apart that differ by less than 4e-6.  Where these are equal the lower beam comes first, and within a beam the logits decide, exactly as they
+// are (beside a score of -1e30 all of a beam's candidates are equal in 64 bits too), then the lower word: a key of 4, 32 and 28 bits.  Latency: 32 requests of eight beams
 // 6 us, one of sixteen beams in 25 parts each 14 (141 when every entry was looked at: the lists are in order, and a line through threads that have
 // entries of every rank is a low one).
 constexpr int kBeamLists = 4 * 148 + kBeamMax;            // lists of a request at most: parts of all rows, or one of each
@@ -330,7 +335,7 @@ __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned 
     int* parent = (int*)a[1] + (size_t)vb * K;
     float* score_out = (float*)a[2] + (size_t)vb * K;
     int* live_out = (int*)a[3] + (size_t)vb * K;
-    BeamRoom<double>& s = *reinterpret_cast<BeamRoom<double>*>(smem);
+    BeamRoom<double, BeamKey>& s = *reinterpret_cast<BeamRoom<double, BeamKey>*>(smem);
     // of a beam: its logits' maximum, the logarithm of the sum of exponentials below it, its score.  Applied one after the other: their sum
     // would lose the smaller ones where the logits are at the type's lowest value.
     double* log_sum = reinterpret_cast<double*>(smem + kBeamSmem);
@@ -369,17 +374,19 @@ __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned 
         }
     }
     __syncthreads();
-    // a list's i-th entry: the value, -infinity for none, and the place among the request's candidates
+    // a list's i-th entry: the value, -infinity for none, and its key
     const int lists = K * p.parts;
-    auto entry = [&](int list, int i, int* at) -> double {
+    auto key_of = [](int b, unsigned order, int w) { return (BeamKey)b << 60 | (BeamKey)order << 28 | (unsigned)w; };
+    auto entry = [&](int list, int i, BeamKey* at) -> double {
         const int b = list / p.parts;
         const float* x = parts + (size_t)list * F + 2 + i;
         const float v = x[0];
-        *at = b * p.vocab + min(max(__float_as_int(x[K]), 0), p.vocab - 1);
+        const unsigned bits = __float_as_uint(v + 0.f);          // (-0 as 0), ascending as the logits descend:
+        *at = key_of(b, bits >> 31 ? bits : ~bits & 0x7fffffffu, min(max(__float_as_int(x[K]), 0), p.vocab - 1));
         return kind[b] == 1 ? (double)v - highest[b] - log_sum[b] + base[b] : -INFINITY;
     };
-    auto take = [&](int i, double v, int at) {
-        const int b = at / p.vocab, w = at - b * p.vocab;
+    auto take = [&](int i, double v, BeamKey at) {
+        const int b = (int)(at >> 60), w = (int)(at & 0xfffffffu);
         token[i] = w;
         parent[i] = vb * K + b;
         score_out[i] = (float)v;
@@ -388,36 +395,37 @@ __device__ __forceinline__ bool body_beam_pick(const KTask& t, int vb, unsigned 
     // K first entries reach the line: only lists whose first entries do are looked into
     const double own = tid < K && kind[tid] == 2 ? (double)score[tid] : -INFINITY;
     double top = own;
-    int at;
+    BeamKey at;
+    const BeamKey own_at = key_of(tid & 15, 0, p.eos);           // (its beam's only candidate)
     for (int c = tid; c < lists; c += kThreads) {
         heads[c] = entry(c, 0, &at);
         top = fmax(top, heads[c]);
     }
     if (tid == 0) *walked = 0;
-    const double line = block_line<double>(K, s, top);
+    const double line = block_line(K, s, top);
     for (int c = tid; c < lists; c += kThreads)
         if (heads[c] >= line && heads[c] > -INFINITY) which[atomicAdd(walked, 1)] = c;
     __syncthreads();
     const int entries = *walked * K;
-    block_collect<double>(s, [&](auto f) {
+    block_collect(s, [&](auto f) {
 #pragma unroll 2
         for (int c = tid; c < entries; c += kThreads) {
             const int list = c / K;
             const double v = entry(which[list], c - list * K, &at);
             if (v >= line) f(v, at);
         }
-        if (own >= line) f(own, tid * p.vocab + p.eos);
+        if (own >= line) f(own, own_at);
     });
     __syncthreads();
     const int n = s.count;
-    const int found = n <= kBeamRoom ? block_place<double>(K, s, n, take) : block_top<double>(K, s,
+    const int found = n <= kBeamRoom ? block_place(K, s, n, take) : block_top(K, s,
         [&](auto f) {
             for (int c = tid; c < lists * K; c += kThreads) {
                 const int list = c / K;
                 const double v = entry(list, c - list * K, &at);
                 f(v, at);
             }
-            f(own, tid * p.vocab + p.eos);
+            f(own, own_at);
         }, take);
     if (tid >= found && tid < K) {
         token[tid] = -1;

@@ -323,8 +323,8 @@ def beam_select(logits, score, live, *, beams: int, eos: int, start=None, out=No
     token counts.  ``score`` [rows] fp32: sums of log-probabilities; ``live`` [rows] int32: 0 for beams that have ended, which compete with their
     score and the word ``eos``.  rows = requests * beams, the beams of a request side by side.
 
-    Returns (token, parent, score, live) of the new beams, best first, int32 but for the score; equal candidates by the lowest
-    beam * vocab + word.  ``parent`` is a row, as ``page_tables`` wants it, and ``live`` (0 or 1) is what each row adds in the next step.  Where a
+    Returns (token, parent, score, live) of the new beams, best first, int32 but for the score.  Candidates are compared in 64 bits; of equal ones
+    the lower beam's come first, and of one beam's those of the greater logits, then of the lower words.  ``parent`` is a row, as ``page_tables`` wants it, and ``live`` (0 or 1) is what each row adds in the next step.  Where a
     request has fewer candidates above -infinity than beams, the rest are token -1, parent -1, score -infinity, live 0: a row of logits with a
     NaN, an infinity or nothing but -infinity has none, nor has a beam whose score is not finite.
     """

@@ -26,3 +26,45 @@ def test_many_tokens_over_a_long_table(T):
     want, size = attend_by_hand(q[some], kc, vc, table, tok[some])
     assert ((got[some] - want).abs() <= ATTEND_TOL * size + 2.0 ** -24 * size.amax()).all()
     assert not got[tok[:, 2] == 0].any() and capi.device_error() == 0
+
+
+# ---- beam selection: candidates that are equal in 64 bits ------------------------------------------------------------------------
+def check_order(logits, score, live, K, eos):
+    """Sorted by the value in 64 bits, then the beam, the logit as it is, the word."""
+    x, token, parent = logits.double().cpu().numpy(), [], []
+    for a in range(0, len(x), K):
+        found = []
+        for b in range(a, a + K):
+            if live[b] == 0:
+                found.append((-float(score[b]), b, 0.0, eos))
+                continue
+            top = x[b].max()
+            c = float(score[b]) + (x[b] - top - np.log(np.exp(x[b] - top).sum()))
+            best = np.lexsort((np.arange(len(c)), -x[b], -c))[:K]
+            found += [(-c[w], b, -x[b][w], w) for w in best]
+        for _, b, _, w in sorted(found)[:K]:
+            token.append(w)
+            parent.append(b)
+    got = decode.beam_select(logits, score, live, beams=K, eos=eos)
+    assert got[0].tolist() == token and got[1].tolist() == parent
+
+
+@pytest.mark.parametrize("V", [300, 30000, 100003])
+@pytest.mark.parametrize("K", [3, 8, 16])
+def test_equal_candidates_go_by_their_logits(K, V):
+    g = torch.Generator("cuda").manual_seed(V + K)
+    live = torch.ones(2 * K, device="cuda", dtype=I)
+    # logits far below 64 bits of the highest one
+    logits = 1e-20 * torch.randn(2 * K, V, device="cuda", generator=g)
+    logits[:, V // 2] = 100.0
+    check_order(logits, torch.zeros(2 * K, device="cuda"), live, K, 2)
+    # scores beside which the logits do not count, of live beams and of one that has ended
+    logits = torch.randn(2 * K, V, device="cuda", generator=g)
+    score = torch.full((2 * K,), -3e38, device="cuda")
+    check_order(logits, score, live, K, 2)
+    live[K + 1] = 0
+    score[:K - 1] = -3.1e38
+    check_order(logits, score, live, K, 2)
+    # zeros of either sign are equal, and so are more than are ranked side by side
+    logits = torch.where(torch.rand(2 * K, V, device="cuda", generator=g) < 0.5, 0.0, -0.0)
+    check_order(logits, score, live, K, 2)
