@@ -331,15 +331,15 @@ struct PagedSimt {
 // ---- tensor cores -----------------------------------------------------------------------------------------------------------
 // From three query heads to a key head on, the multiplications of the fp32 form are what takes the time (64 rows of 32 heads over 8 as above:
 // 375 us); 16-bit keys and values are operands of mma.sync as they are.  Queries and probabilities keep their 32 bits: a bf16 query is the
-// exact sum of three bf16 values, an fp16 one that of two fp16 values, scaled to the type's range, but for 2^-22 of it.  The sixteen rows of
-// a multiplication hold four or eight heads' parts side by side, so that one instruction, or two, multiplies all of them.  Sums are carried on
-// outside the tensor core, whose additions truncate.
+// exact sum of three bf16 values, an fp16 one that of two fp16 values, scaled to the type's range, but for 2^-22 of it or 2^-39 of the
+// largest.  The sixteen rows of a multiplication hold four or eight heads' parts side by side, so that one instruction, or two, multiplies
+// all of them.  Sums are carried on outside the tensor core, whose additions truncate.
 // A warp takes 16 keys at a time, from its ring into registers in the operands' layout: lane (g, c) has 16-byte pieces of keys g and 8 + g,
 // whose eight dimensions are its K positions of two instructions; and of the values of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 eight dimensions,
 // which are its columns of eight instructions.  These multiplications keep the tensor pipe 28 % busy while HBM is the bound, so that the
 // 128 rows of a tcgen05 tile would wait for the same bytes.
 // What the parts cannot carry (an infinity or NaN among the operands) ends as a sum that is not finite: such a range is worked out again by
-// fp32 instructions.
+// fp32 instructions, as is one whose queries are of sizes that two fp16 values cannot hold side by side.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -378,7 +378,7 @@ template <> struct Rows<__half, 8> {
         lo = *reinterpret_cast<const uint32_t*>(&a);
         hi = *reinterpret_cast<const uint32_t*>(&b);
     }
-    // a probability of 1 becomes 2^15: two fp16 values have 22 bits of it down to 2^-18
+    // a probability of 1 becomes 2^15: two fp16 values have 22 bits of it down to 2^-18; of smaller ones 2^-40 is lost at most
     static constexpr float kLift = 15.f;
     static constexpr bool kScaled = true, kHalves = false;
 };
@@ -481,17 +481,30 @@ struct PagedMma {
         float back = 1.f;           // what scores are multiplied by
         {
             float4 x[KS];
-            float high = 0.f;
+            float high = 0.f, low = INFINITY;
+            auto least = [&](float y) { low = y != 0.f ? fminf(low, fabsf(y)) : low; };
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 x[ks] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (head < r.heads) x[ks] = *reinterpret_cast<const float4*>(r.q + head * D + (c + 4 * (ks >> 1)) * 8 + (ks & 1) * 4);
-                if (A::kScaled) high = fmaxf(fmaxf(fmaxf(high, fabsf(x[ks].x)), fmaxf(fabsf(x[ks].y), fabsf(x[ks].z))), fabsf(x[ks].w));
+                if (A::kScaled) {
+                    high = fmaxf(fmaxf(fmaxf(high, fabsf(x[ks].x)), fmaxf(fabsf(x[ks].y), fabsf(x[ks].z))), fabsf(x[ks].w));
+                    least(x[ks].x); least(x[ks].y); least(x[ks].z); least(x[ks].w);
+                }
             }
             float by = scale;
             if (A::kScaled) {
                 high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
                 high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                // What the largest leaves of the others: 2^-39 of it.  Up to 1024 that is 2^-29, which a key would have to be
+                // in the thousands for to be seen; beyond, where there are others that it takes bits from, the range is
+                // worked out by fp32 instructions.
+                if (__any_sync(0xffffffffu, high > 1024.f && low < high * 0x1p-17f)) {
+                    copy_wait<0>();
+                    __syncwarp();
+                    lost = true;
+                    return true;
+                }
                 // the largest query becomes 2^14 to 2^15
                 const int up = min(max(14 - ilogbf(fmaxf(high, 1e-36f)), -110), 110);
                 by = ldexpf(1.f, up);

@@ -5,7 +5,7 @@ import torch
 
 from reef_b200 import capi, decode
 from reef_b200.resources import decoding
-from test_gpu_decode import ATTEND_TOL, F, I, attend_by_hand, attend_inputs, dev
+from test_gpu_decode import ATTEND_TOL, F, I, attend_by_hand, attend_inputs, check_attention, dev
 
 pytestmark = pytest.mark.gpu
 TYPES = [F, torch.bfloat16, torch.float16]
@@ -68,3 +68,16 @@ def test_equal_candidates_go_by_their_logits(K, V):
     # zeros of either sign are equal, and so are more than are ranked side by side
     logits = torch.where(torch.rand(2 * K, V, device="cuda", generator=g) < 0.5, 0.0, -0.0)
     check_order(logits, score, live, K, 2)
+
+
+# ---- attention: queries of very different sizes ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("D,H,kv", [(64, 8, 1), (128, 6, 2), (256, 16, 2), (64, 4, 4)])
+@pytest.mark.parametrize("M", [8, 400])
+@pytest.mark.parametrize("size", [1000.0, 1e5, 1e8, 1e12, 1e30])
+def test_a_large_query_beside_a_key_of_zero(type, D, H, kv, M, size):
+    """One dimension in which the keys are zero: the score is what the others say, whatever the query holds there."""
+    q, kc, vc, table, tok = attend_inputs(np.random.default_rng([D, H]), [100, 120, 1, 128], H, kv, D, 16, M, type)
+    kc[..., 9] = torch.where(kc[..., 9].isnan(), kc[..., 9], 0.0)
+    q[:3, :, 9] = size
+    check_attention(q, kc, vc, table, tok)
