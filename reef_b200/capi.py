@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import threading
+import weakref
 
 import numpy as np
 
@@ -159,20 +159,17 @@ def _buf(a: np.ndarray):
 class Kernel:
     """One kernel of the registry on device pointers (``reef_module_get_kernel`` / ``reef_launch``): for programs that hold their own
     device memory.  Resolving a name needs no GPU.  ``prepare`` does a device's one-time work and has to run ahead of the first launch
-    there, outside a stream capture; launches are asynchronous and may be captured."""
-
-    _module, _lock = None, threading.Lock()
+    there, outside a stream capture; launches are asynchronous and may be captured.  (What is launched holds a copy of what it needs: the object
+    may go while the kernel runs.)"""
 
     def __init__(self, name: str):
         self._lib = lib = cuda_lib()
         self.name, self._h = name, C.c_void_p()
-        with Kernel._lock:      # a module is a list of its kernels
-            if Kernel._module is None:
-                module = C.c_void_p()
-                _check(lib.reef_module_open(None, C.byref(module)), "reef_module_open")
-                lib.reef_launch.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]
-                Kernel._module = module
-            _check(lib.reef_module_get_kernel(Kernel._module, name.encode(), C.byref(self._h)), f"reef_module_get_kernel({name})")
+        module = C.c_void_p()
+        _check(lib.reef_module_open(None, C.byref(module)), "reef_module_open")
+        weakref.finalize(self, lib.reef_module_close, module).atexit = False
+        lib.reef_launch.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]
+        _check(lib.reef_module_get_kernel(module, name.encode(), C.byref(self._h)), f"reef_module_get_kernel({name})")
         self._dims, smem, nargs = (C.c_uint32 * 6)(), C.c_uint32(), C.c_int()
         _check(lib.reef_kernel_geometry(self._h, self._dims, C.byref(smem), C.byref(nargs)), "reef_kernel_geometry")
         self._smem, self.num_args = smem.value, nargs.value

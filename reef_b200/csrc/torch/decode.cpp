@@ -2,7 +2,8 @@
 // outputs and workspace, launches.  In Python this took 20 us a call, more than most of the kernels; here 4 to 7.
 //
 // A signature is the operator, its whole-number options, and type, device, sizes and strides of every tensor.  Nothing of a tensor's
-// identity or contents is kept.
+// identity or contents is kept.  The last kMaxPlans signatures are: a server whose prompts have every length would else fill its memory with
+// them; one that is asked for again is defined again.
 #include <ATen/ops/empty.h>
 #include <Python.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -11,6 +12,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <deque>
+#include <memory>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -36,7 +39,12 @@ struct Plan {
     std::vector<int> aligned;                   // tensors that begin at a 16-byte boundary
     std::vector<std::pair<int, int>> apart;     // tensors that do not lie over each other
     size_t workspace;
+    PyObject* owner = nullptr;                  // keeps the kernels (everything here runs under the interpreter's lock)
+    Plan() = default;
+    Plan(const Plan&) = delete;
+    ~Plan() { Py_XDECREF(owner); }
 };
+constexpr size_t kMaxPlans = 4096;
 typedef std::vector<int64_t> Key;
 struct Hash {
     size_t operator()(const Key& k) const {
@@ -45,8 +53,12 @@ struct Hash {
         return (size_t)(h ^ (h >> 29));
     }
 };
-std::unordered_map<Key, Plan, Hash>* plans() {
-    static auto* p = new std::unordered_map<Key, Plan, Hash>;     // (never freed: kernels outlive the interpreter's modules)
+struct Plans {
+    std::unordered_map<Key, std::shared_ptr<const Plan>, Hash> of;
+    std::deque<Key> order;      // the oldest first
+};
+Plans* plans() {
+    static auto* p = new Plans;     // (never freed: nothing is given back to an interpreter that has ended)
     return p;
 }
 
@@ -129,9 +141,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             PyErr_Clear();
             Py_RETURN_NONE;
         }
-        auto it = plans()->find(c.key);
-        if (it == plans()->end()) Py_RETURN_NONE;
-        const Plan& p = it->second;
+        auto it = plans()->of.find(c.key);
+        if (it == plans()->of.end() || c.n == 0 || c.t[0] == nullptr) Py_RETURN_NONE;
+        const std::shared_ptr<const Plan> plan = it->second;        // (an allocation may run other code, which may define others)
+        const Plan& p = *plan;
         if (c10::GradMode::is_enabled())
             for (int i = 0; i < c.n; i++)
                 if (c.t[i] && c.t[i]->requires_grad())
@@ -202,11 +215,11 @@ bool numbers(PyObject* o, std::vector<int64_t>* out) {
     return true;
 }
 
-// define(operator, inputs, outputs, options, launches, allocate, workspace, aligned, apart): launches = [(handle, dims, smem, args)], allocate =
-// [(type of input i or -1 for int32, sizes)]
+// define(operator, inputs, outputs, options, launches, allocate, workspace, aligned, apart, owner): launches = [(handle, dims, smem, args)],
+// allocate = [(type of input i or -1 for int32, sizes)], owner: what has to live as long as the handles are used
 PyObject* define(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-    if (nargs != 9) {
-        PyErr_SetString(PyExc_TypeError, "define: nine arguments");
+    if (nargs != 10) {
+        PyErr_SetString(PyExc_TypeError, "define: ten arguments");
         return nullptr;
     }
     try {
@@ -215,7 +228,8 @@ PyObject* define(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             PyErr_SetString(PyExc_TypeError, "define: not a signature");
             return nullptr;
         }
-        Plan p;
+        const std::shared_ptr<Plan> made = std::make_shared<Plan>();
+        Plan& p = *made;
         for (Py_ssize_t i = 0; i < PyList_Size(args[4]); i++) {
             PyObject* l = PyList_GetItem(args[4], i);
             std::vector<int64_t> one, dims, a;
@@ -241,7 +255,24 @@ PyObject* define(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if (PyErr_Occurred() || !numbers(args[7], &aligned) || !numbers(args[8], &apart)) return nullptr;
         for (int64_t i : aligned) p.aligned.push_back((int)i);
         for (size_t i = 0; i + 1 < apart.size(); i += 2) p.apart.emplace_back((int)apart[i], (int)apart[i + 1]);
-        (*plans())[c.key] = std::move(p);
+        Py_INCREF(args[9]);
+        p.owner = args[9];
+        Plans* all = plans();
+        std::shared_ptr<const Plan> gone = made;            // given up at the end, when what that runs finds everything in order
+        auto at = all->of.find(c.key);
+        if (at != all->of.end()) {
+            at->second.swap(gone);
+        } else {
+            all->order.push_back(c.key);
+            all->of.emplace(c.key, made);
+            gone.reset();
+            if (all->of.size() > kMaxPlans) {
+                at = all->of.find(all->order.front());
+                gone.swap(at->second);
+                all->of.erase(at);
+                all->order.pop_front();
+            }
+        }
         Py_RETURN_NONE;
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -249,8 +280,11 @@ PyObject* define(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
+PyObject* count(PyObject*, PyObject*) { return PyLong_FromSize_t(plans()->of.size()); }
+
 PyMethodDef methods[] = {{"call", (PyCFunction)(void (*)())call, METH_FASTCALL, nullptr},
                          {"define", (PyCFunction)(void (*)())define, METH_FASTCALL, nullptr},
+                         {"count", count, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_decode", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -62,7 +62,8 @@ def page_state(rows: int, max_pages: int, tokens: int, *, fork: bool = False, de
 
 
 # ---- checks and launches -------------------------------------------------------------------------------------------------
-# A signature (types, devices, sizes, strides, options) is checked and resolved here, once; from then on _decode.call does everything.
+# A signature (types, devices, sizes, strides, options) is checked and resolved here, once; from then on _decode.call does everything, for the
+# last 4096 of them.
 _TABLES, _APPEND, _ATTENTION, _BEAMS = range(4)
 _ready = set()      # devices whose kernels are set up
 _lock = threading.Lock()
@@ -152,7 +153,7 @@ def _define(op, inputs, outputs, options, kernels, args, allocate, workspace, al
     """``args``: per kernel the tensors of its arguments, by position among inputs and outputs, -1 the workspace; ``allocate``: (input whose type
     it has or -1 for int32, shape) per output; ``apart``: (position, positions that it must not lie over)."""
     _decode.define(op, inputs, outputs, options, [(k.handle, k.dims, k.dyn_smem, a) for k, a in zip(kernels, args)], allocate, workspace, aligned,
-                   [x for i, others in apart for j in others for x in (i, j)])
+                   [x for i, others in apart for j in others for x in (i, j)], kernels)
 
 
 # ---- operators -------------------------------------------------------------------------------------------------------------

@@ -118,3 +118,31 @@ def test_sizes_beyond_the_kernels_are_named():
     assert "not on a GPU" in beams() and "not on a GPU" in beams(rows=1 << 20)
     assert "words: " in beams(words=1 << 27)
     assert "rows: 1048577" in beams(rows=(1 << 20) + 1)
+
+
+def test_signatures_and_kernels_do_not_pile_up():
+    """A server whose prompts have every length: what is kept of them has a bound."""
+    r = _run("""
+import resource, torch, weakref
+from reef_b200 import capi, decode
+native = decode._decode
+native.count()
+native = decode._decode
+seen = []
+def many(first, n):
+    for i in range(first, first + n):
+        k = capi.Kernel(f"reef_paged_append__tokens{i + 1}_kvh1_d64_ps16_pages8_kt0")
+        native.define(99, (None,), None, (i,), [(k.handle, k.dims, k.dyn_smem, [0])], [], 0, [], [], [k])
+        seen.append(weakref.ref(k))
+many(0, 6000)
+assert native.count() == 4096 and native.call(99, (None,), None, (1,)) is None
+alive = [i for i, k in enumerate(seen) if k() is not None]
+assert 4096 <= len(alive) <= 4097 and alive[0] >= 1903, (len(alive), alive[0])
+before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+many(6000, 60000)
+assert native.count() == 4096
+print("kept", resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 24 << 10)
+native.define(99, (None,), None, (65999,), [], [], 0, [], [], [])      # one that is there is replaced
+assert native.count() == 4096
+""")
+    assert r.stdout.strip() == "kept True", r.stdout + r.stderr

@@ -81,3 +81,28 @@ def test_a_large_query_beside_a_key_of_zero(type, D, H, kv, M, size):
     kc[..., 9] = torch.where(kc[..., 9].isnan(), kc[..., 9], 0.0)
     q[:3, :, 9] = size
     check_attention(q, kc, vc, table, tok)
+
+
+# ---- signatures that have been given up ------------------------------------------------------------------------------------------
+def test_more_signatures_than_are_kept():
+    """A call whose signature has been given up is defined again; a graph that it was captured in goes on."""
+    q, kc, vc, table, tok = attend_inputs(np.random.default_rng(3), [500, 3000, 1], 8, 2, 64, 16, 400, torch.bfloat16)
+    table, tok = dev(table, I), dev(tok, I)
+    want = decode.paged_attention(q, kc, vc, table, tok)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = decode.paged_attention(q, kc, vc, table, tok)
+    logits, score, live = torch.randn(2, 5000, device="cuda"), torch.zeros(2, device="cuda"), torch.tensor([0, 1], device="cuda", dtype=I)
+    first = decode.beam_select(logits, score, live, beams=2, eos=0)
+    for eos in range(1, 4300):
+        last = decode.beam_select(logits, score, live, beams=2, eos=eos)
+        if eos == 2000:
+            torch.cuda.synchronize()
+    assert decode._decode.count() == 4096
+    assert last[0][0].item() == 4299 and first[0][0].item() == 0
+    again = decode.beam_select(logits, score, live, beams=2, eos=0)
+    assert all(torch.equal(a, b) for a, b in zip(again, first))
+    got.zero_()
+    graph.replay()
+    assert torch.equal(got, want) and torch.equal(decode.paged_attention(q, kc, vc, table, tok), want)
+    assert capi.device_error() == 0
