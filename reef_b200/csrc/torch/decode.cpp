@@ -8,6 +8,7 @@
 #include <Python.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -149,6 +150,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             for (int i = 0; i < c.n; i++)
                 if (c.t[i] && c.t[i]->requires_grad())
                     return PyUnicode_FromString("inputs require gradients and there is no backward pass (use torch.no_grad)");
+        if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+            for (int i = 0; i < c.n; i++)
+                if (c.t[i] && c.t[i]->_fw_grad(0).defined())
+                    return PyUnicode_FromString("inputs carry tangents and there is no forward-mode derivative");
         const c10::cuda::CUDAGuard guard(c.t[0]->device());
         at::Tensor fresh[kMaxTensors];
         if (!c.made)

@@ -14,7 +14,7 @@ stream capture (it sets up the kernels there); with other shapes later calls may
 
 Arguments are refused with ``ReefError`` (OutOfRange) before anything is launched.  Values on the device (lengths, ids, slots) are
 not looked at by the host: the kernels bound every one of them.  There is no backward pass: inputs that require gradients are refused
-while gradients are recorded.
+while gradients are recorded, and so are those that carry forward-mode tangents.
 """
 from __future__ import annotations
 
@@ -86,6 +86,10 @@ def _inference(what, *tensors):
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:
                 _refuse(what, "inputs require gradients and there is no backward pass (use torch.no_grad)")
+    if torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                _refuse(what, "inputs carry tangents and there is no forward-mode derivative")
 
 
 def _want(what, name, t, shape, dtype=torch.int32, device=None, dense=True):

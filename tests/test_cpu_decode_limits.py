@@ -146,3 +146,14 @@ native.define(99, (None,), None, (65999,), [], [], 0, [], [], [])      # one tha
 assert native.count() == 4096
 """)
     assert r.stdout.strip() == "kept True", r.stdout + r.stderr
+
+
+def test_inputs_that_carry_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    f = torch.float32
+    c = torch.zeros(8, 1, 16, 64)
+    with fw.dual_level(), torch.no_grad():
+        q = fw.make_dual(torch.zeros(2, 1, 64), torch.ones(2, 1, 64))
+        for call in (lambda x: decode.paged_attention(x, c, c, _big(2, 4), _big(2, 4)), lambda x: decode.paged_append(x, x, _big(2, 4), c, c.clone()),
+                     lambda x: decode.beam_select(x[:, 0], x[:, 0, 0], _big(2), beams=1, eos=0)):
+            assert "tangents" in _why(call, q) and "not on a GPU" in _why(call, fw.unpack_dual(q).primal)

@@ -106,3 +106,15 @@ def test_more_signatures_than_are_kept():
     graph.replay()
     assert torch.equal(got, want) and torch.equal(decode.paged_attention(q, kc, vc, table, tok), want)
     assert capi.device_error() == 0
+
+
+def test_tangents_are_refused_by_a_known_signature_too():
+    import torch.autograd.forward_ad as fw
+    q, kc, vc, table, tok = attend_inputs(np.random.default_rng(3), [50, 3], 4, 2, 64, 16, 4, F)
+    table, tok = dev(table, I), dev(tok, I)
+    want = decode.paged_attention(q, kc, vc, table, tok)
+    for _ in range(2):
+        with fw.dual_level():
+            with pytest.raises(capi.ReefError, match="tangents"):
+                decode.paged_attention(fw.make_dual(q, torch.ones_like(q)), kc, vc, table, tok)
+            assert torch.equal(decode.paged_attention(q, kc, vc, table, tok), want)
