@@ -83,7 +83,7 @@ bool collect(PyObject* tuple, Call* c) {
         }
         if (!THPVariable_Check(o)) return false;
         const at::Tensor& t = THPVariable_Unpack(o);
-        if (!t.is_cuda() || t.layout() != at::kStrided) return false;
+        if (!t.is_cuda() || t.layout() != at::kStrided || t.is_neg()) return false;
         c->t[c->n++] = &t;
         c->key.push_back((int64_t)t.scalar_type() << 16 | (int64_t)t.get_device() << 8 | t.dim());
         for (int64_t s : t.sizes()) c->key.push_back(s);

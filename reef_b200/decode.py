@@ -99,6 +99,8 @@ def _want(what, name, t, shape, dtype=torch.int32, device=None, dense=True):
         _refuse(what, f"{name} is {t.dtype}, not {dtype}")
     if tuple(t.shape) != tuple(shape):
         _refuse(what, f"{name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
+    if t.is_neg():
+        _refuse(what, f"{name} is a view that stands for its negative (resolve_neg makes it a tensor of its own)")
     if not t.is_cuda:
         _refuse(what, f"{name} is on {t.device}, not on a GPU")
     if device is not None and t.device != device:

@@ -157,3 +157,15 @@ def test_inputs_that_carry_tangents_are_refused():
         for call in (lambda x: decode.paged_attention(x, c, c, _big(2, 4), _big(2, 4)), lambda x: decode.paged_append(x, x, _big(2, 4), c, c.clone()),
                      lambda x: decode.beam_select(x[:, 0], x[:, 0, 0], _big(2), beams=1, eos=0)):
             assert "tangents" in _why(call, q) and "not on a GPU" in _why(call, fw.unpack_dual(q).primal)
+
+
+def test_views_that_stand_for_their_negative_are_refused():
+    """The imaginary part of a conjugate holds the values of the other sign."""
+    c, q = torch.zeros(8, 1, 16, 64), torch.zeros(2, 1, 64)
+    score = torch.zeros(1, dtype=torch.complex64).conj().imag
+    assert score.is_neg() and score.is_contiguous()
+    neg = torch._neg_view
+    assert "negative" in _why(decode.paged_attention, q, neg(c), c, _big(2, 4), _big(2, 4))
+    assert "negative" in _why(decode.paged_append, q, q, _big(2, 4), neg(c), c)
+    assert "negative" in _why(decode.page_tables, neg(_big(2, 4).clone()), _big(2), _big(2), pages=8, page_size=16, tokens=2)
+    assert "negative" in _why(decode.beam_select, neg(torch.zeros(1, 9)), torch.zeros(1), _big(1), beams=1, eos=0)

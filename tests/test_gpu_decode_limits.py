@@ -118,3 +118,13 @@ def test_tangents_are_refused_by_a_known_signature_too():
             with pytest.raises(capi.ReefError, match="tangents"):
                 decode.paged_attention(fw.make_dual(q, torch.ones_like(q)), kc, vc, table, tok)
             assert torch.equal(decode.paged_attention(q, kc, vc, table, tok), want)
+
+
+def test_views_that_stand_for_their_negative_are_refused():
+    logits, live = torch.randn(1, 50, device="cuda"), torch.ones(1, device="cuda", dtype=I)
+    score = torch.full((1,), 3 - 7j, device="cuda").conj().imag            # 7, in memory -7
+    assert score.is_neg() and score.is_contiguous()
+    decode.beam_select(logits, score.resolve_neg(), live, beams=1, eos=0)
+    for _ in range(2):
+        with pytest.raises(capi.ReefError, match="negative"):
+            decode.beam_select(logits, score, live, beams=1, eos=0)
