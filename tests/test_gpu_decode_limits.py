@@ -128,3 +128,61 @@ def test_views_that_stand_for_their_negative_are_refused():
     for _ in range(2):
         with pytest.raises(capi.ReefError, match="negative"):
             decode.beam_select(logits, score, live, beams=1, eos=0)
+
+
+# ---- attention: the keys of all rows divided among blocks, more tokens than a warp has lanes, and than a block has threads ---------------
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("H,kv,D", [(2, 2, 64), (8, 1, 64), (6, 2, 128), (10, 1, 128), (3, 1, 256)])
+@pytest.mark.parametrize("T", [32, 33, 256, 257, 600])
+def test_division_of_many_tokens(type, H, kv, D, T):
+    R, S, M = 7, 16, 4096
+    assert len(decoding.paged_attention(T, R, H, kv, D, S, M, 100, {F: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16"}[type])) == 2
+    rng = np.random.default_rng([T, H, D])
+    lens = np.array([700, 0, 1, 16, 333, 17, 512])
+    _, kc, vc, table, _ = attend_inputs(rng, lens, H, kv, D, S, M, type)
+    q = torch.randn(T, H, D, device="cuda")
+    for kind in range(3):
+        tok = np.zeros((T, 4), int)
+        tok[:, 1] = rng.integers(0, R, T) if kind else np.arange(T) * R // T
+        tok[:, 2] = lens[tok[:, 1]]
+        if kind == 1:                                       # any length up to the row's; tokens without a row
+            tok[:, 2] = rng.integers(0, tok[:, 2] + 1)
+            tok[rng.random(T) < 0.1, 1] = -1
+            tok[T // 3, 1] = R
+        if kind == 2:                                       # runs of tokens without keys, at both ends and between
+            tok[: T // 4, 2] = 0
+            tok[T // 2:T // 2 + T // 5, 2] = -3
+            tok[-T // 8:, 2] = 0
+        out = torch.full((T, H, D), 7.0, device="cuda")
+        got = check_attention(q, kc, vc, table, tok, out=out)
+        assert not got[(tok[:, 2] <= 0) | (tok[:, 1] < 0) | (tok[:, 1] >= R)].any()
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_division_of_a_single_row_among_many_tokens(type):
+    """One token with keys among hundreds without, wherever it stands."""
+    T, H, kv, D, S, M = 300, 8, 2, 64, 16, 4096
+    q, kc, vc, table, _ = attend_inputs(np.random.default_rng(1), [30000], H, kv, D, S, M, type)
+    q = torch.randn(T, H, D, device="cuda")
+    for at in (0, 1, 255, 256, 299):
+        tok = np.zeros((T, 4), int)
+        tok[:, 1] = -1
+        tok[at] = 0, 0, 30000, 0
+        got = check_attention(q, kc, vc, table, tok, out=torch.full((T, H, D), 7.0, device="cuda"))
+        assert got[at].any() and not got[np.arange(T) != at].any()
+
+
+# ---- attention: the largest queries ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("H,kv", [(2, 2), (8, 1), (6, 2)])
+@pytest.mark.parametrize("M", [8, 400])
+@pytest.mark.parametrize("size", [3e38, -3e38])
+def test_the_largest_queries(type, H, kv, M, size):
+    """3e38 times a key of 4 is within fp32 once it is scaled by log2 e / 8, and a single key, or equal ones, have all the weight: scores of keys
+    that differ there are 1e29 apart or more, and what the other dimensions say is lost in 32 and in 64 bits alike.  Beside keys of zero it counts."""
+    q, kc, vc, table, tok = attend_inputs(np.random.default_rng(6), [100, 120, 1], H, kv, 64, 16, M, type)
+    kc[..., 9] = torch.where(kc[..., 9].isnan(), kc[..., 9], kc[..., 9].clamp(-4, 4))
+    q[0, 0, 9] = size
+    check_attention(q, kc, vc, table, tok)
+    kc[..., 9] = torch.where(kc[..., 9].isnan(), kc[..., 9], 0.0)
+    check_attention(q, kc, vc, table, tok)
