@@ -40,7 +40,7 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // that is partly filled and that a lower row with the same parent keeps, and `fork` says what is to be copied into it.  So no
 // two rows ever share a page that one of them will write.  Free is what no row keeps; lowest ids first, rows in their order.
 // A row that cannot be served is refused (status 2: lengths, parent or ids out of range; 3: more than `tokens` new tokens in all;
-// 1: no pages left) and comes out empty.  Tokens are counted over the rows that are not 2, and all of them are 3 from the one on that
+// 1: no pages left) and comes out empty.  With 1 and 3 what it kept stays in use in this step, with 2 it keeps nothing.  Tokens are counted over the rows that are not 2, and all of them are 3 from the one on that
 // goes beyond; pages over the rows left, and those that need any are 1 from the one on that goes beyond.
 // The state goes from one set of buffers into another, so the kernel can be run again after a preemption.
 //

@@ -174,8 +174,15 @@ def page_tables(table, lens, new, *, pages: int, page_size: int, tokens: int, pa
     A row gets free pages, lowest id first, where its tokens need them.  Rows that go on from the same parent share its full pages; a last
     page that is partly filled stays with the lowest of them, and ``fork`` names the copies that the others need (``paged_append`` makes
     them).  Rows may come in with shared pages as long as these are full.  An id of -1 stands for a page that has been given up
-    (``paged_attention`` leaves its tokens out).  Rows that cannot be served are refused by ``status`` and come out empty; the old state is
-    still there, as ``out`` may not lie over it.
+    (``paged_attention`` leaves its tokens out).
+
+    Rows that cannot be served are refused by ``status`` and come out empty; the old tables are still there, as ``out`` may not lie over them.
+    Where pages or tokens ran out (1, 3) the old pages are too: no row gets them in this step, and the row can be tried again from the old
+    state.  A row whose lengths, parent or ids are out of range (2), one that is to grow beyond max_pages * page_size among them, keeps
+    nothing: its pages are free for other rows at once, and ``paged_append`` will write there.  Whoever wants to keep such a row looks at
+    its length first, or gives it no new tokens.
+
+    Without ``parent`` there is nothing to copy: the state that comes back has no ``fork``, and one that ``out`` has is left as it was.
     """
     inputs, options = (table, lens, new, parent), (pages, page_size, tokens)
     outputs = None if out is None else tuple(out[:5] if parent is None else out)

@@ -186,3 +186,40 @@ def test_the_largest_queries(type, H, kv, M, size):
     check_attention(q, kc, vc, table, tok)
     kc[..., 9] = torch.where(kc[..., 9].isnan(), kc[..., 9], 0.0)
     check_attention(q, kc, vc, table, tok)
+
+
+# ---- page tables: what becomes of a refused row's pages --------------------------------------------------------------------------------
+def _refuse_one(lens, new, tokens=100, pages=8, parent=None):
+    """Two rows of the pages 0, 1 and 2, 3 in a pool of eight, four tokens to a page, four pages to a row."""
+    table = dev([[0, 1, -1, -1], [2, 3, -1, -1]], I)
+    return table, decode.page_tables(table, dev(lens, I), dev(new, I), pages=pages, page_size=4, tokens=tokens, parent=parent)
+
+
+def test_pages_of_refused_rows():
+    # no pages left, or no tokens: the old ones are nobody else's
+    _, s = _refuse_one([8, 8], [4, 5], pages=5)
+    assert s.status.tolist() == [0, 1] and s.table.tolist() == [[0, 1, 4, -1], [-1] * 4] and s.lens.tolist() == [12, 0]
+    _, s = _refuse_one([8, 8], [4, 8], tokens=11)
+    assert s.status.tolist() == [0, 3] and s.table[0].tolist() == [0, 1, 4, -1]
+    # and the row can be tried again from the old state
+    old, s = _refuse_one([8, 8], [0, 4], pages=5)
+    assert s.status.tolist() == [0, 0] and s.table.tolist() == [[0, 1, -1, -1], [2, 3, 4, -1]]
+    # beyond the longest row it keeps nothing: its pages are the first free ones
+    old, s = _refuse_one([8, 8], [9, 8])
+    assert s.status.tolist() == [2, 0] and s.table[1].tolist() == [2, 3, 0, 1] and old[0].tolist() == [0, 1, -1, -1]
+    # but for those that another row goes on from
+    _, s = _refuse_one([8, 8], [9, 8], parent=dev([0, 0], I))
+    assert s.status.tolist() == [2, 0] and s.table[1].tolist() == [0, 1, 2, 3]
+    # given no new tokens it stays
+    _, s = _refuse_one([8, 16], [8, 0])
+    assert s.status.tolist() == [0, 0] and s.lens.tolist() == [16, 16]
+
+
+def test_a_state_without_parents_has_no_copies():
+    out = decode.page_state(2, 4, 100, fork=True)
+    out.fork.fill_(5)
+    table, lens, new = dev([[0, 1, -1, -1], [2, 3, -1, -1]], I), dev([8, 7], I), dev([1, 1], I)
+    s = decode.page_tables(table, lens, new, pages=8, page_size=4, tokens=100, out=out)
+    assert s.fork is None and (out.fork == 5).all() and s.lens.tolist() == [9, 8]
+    s = decode.page_tables(table, lens, new, pages=8, page_size=4, tokens=100, out=out, parent=dev([0, 1], I))
+    assert s.fork is out.fork and s.fork.tolist() == [[-1, -1, 0, 0]] * 2
