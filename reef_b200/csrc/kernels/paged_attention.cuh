@@ -3,10 +3,12 @@
 // the keys of positions whose page id lies outside the cache left out; zeros where nothing is left.  (The reference attends within
 // a sequence only, resource/bert/bert.cu:22-157.)
 //
-// One pass over the keys with a running maximum and sum; every key and value is read once for up to eight query heads.  Bound by HBM where
-// there is much to read: 64 rows of 32 heads over 8, bf16, 128 dimensions, 860 MB in 152 us (5.7 TB/s, 0.88 of the measured copy rate; SMs
-// do not get equal shares of it), 2048 passes of up to 1 MB 185 us (0.89); fp32 in groups of five, 188 MB in 41 us (0.70).  A
-// call with little to read is a chain of latencies: 12 heads of a row of 77 keys 5.0 us, of 1000 14.
+// One pass over the keys with a running maximum and sum; every key and value is read once for up to eight query heads (fp32 with 256
+// dimensions: four), and again for every further eight: 64 rows, 292368 keys of one key head, 128 dimensions, bf16, 8 heads 43 us, 16 64, 64 205;
+// 64 rows of 128 heads over 8 389, of 64 heads 227.  Bound by HBM where there is much to read: 64 rows of 32 heads over 8, bf16, 128 dimensions,
+// 860 MB in 160 us with the join (5.4 TB/s, 0.83 of the measured copy rate; SMs do not get equal shares of it), 2048 passes of up to 1 MB
+// 185 us (0.89); fp32 in groups of five, 2.4 GB in 413 us (0.90), 188 MB in 47 (0.62, dependent steps).  A call with little to read is a
+// chain of latencies: 12 heads of a row of 77 keys 5.0 us, of 1000 14.
 #pragma once
 #include "bf16_split.cuh"
 #include "paged_cache.cuh"
@@ -336,7 +338,7 @@ struct PagedSimt {
 // all of them.  Sums are carried on outside the tensor core, whose additions truncate.
 // A warp takes 16 keys at a time, from its ring into registers in the operands' layout: lane (g, c) has 16-byte pieces of keys g and 8 + g,
 // whose eight dimensions are its K positions of two instructions; and of the values of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 eight dimensions,
-// which are its columns of eight instructions.  These multiplications keep the tensor pipe 28 % busy while HBM is the bound, so that the
+// which are its columns of eight instructions.  These multiplications keep the tensor pipe 19 % busy while HBM is the bound, so that the
 // 128 rows of a tcgen05 tile would wait for the same bytes.
 // What the parts cannot carry (an infinity or NaN among the operands) ends as a sum that is not finite: such a range is worked out again by
 // fp32 instructions, as is one whose queries are of sizes that two fp16 values cannot hold side by side.
@@ -883,8 +885,9 @@ __host__ inline int paged_warps_of_a_pass(const PagedP& p, long long passes, int
     return w;
 }
 // Blocks of the form with parts: what the SMs hold at once, fewer where the longest rows would not give every warp its least work.  (SMs do
-// not get the same share of the memory's bandwidth: of 148 equal shares of 860 MB one was through after 107 us and one after 147.  Two or
-// three times as many blocks, to be taken by whichever SM is free, brought 157 to 152 us, and cost more in further parts and their join.)
+// not get the same share of the memory's bandwidth: of 148 equal shares of 860 MB one was through after 102 us and one after 145.  Two or
+// three times as many blocks, to be taken by whichever SM is free, brought 157 to 152 us with two blocks to an SM, and cost more in
+// further parts and their join.)
 __host__ inline int paged_parts_blocks(const PagedP& p, long long units) {
     const long long want = (units + 8 * kPagedMinUnits - 1) / (8 * kPagedMinUnits), slots = (long long)paged_blocks_per_sm(p) * kSmsPlanned;
     return (int)(want < slots ? want : slots);

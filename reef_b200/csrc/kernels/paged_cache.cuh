@@ -50,7 +50,8 @@ __device__ __forceinline__ int page_of(const PagedP& p, int pos) { return (int)(
 // Used pages are marked in bytes, a window of the pages at a time, and packed to bits: an atomic OR into a word of bits took 1.5 cycles for
 // every id, 53 us for 62500 of them, a byte is a plain store.  A free page is found by its rank (a prefix sum over the threads' words, a walk
 // through one thread's), by whoever needs it.  16 rows of 500 tokens 7 us, 128 beams 12, 256 rows of two million tokens in all (62500 ids)
-// 21 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them).
+// 21 (86 with atomics, rows one after the other, and free pages handed out by the threads whose words hold them), 1024 rows of 524288 in all
+// in a pool of as many, which takes five windows and the ids five times, 444.
 constexpr int kTablesThreads = 2 * kThreads;
 constexpr int kTablesMaxRows = 1024, kTablesMaxPages = 1 << 19;
 __host__ __device__ constexpr int tables_fixed(int rows, int pages) {
@@ -378,8 +379,9 @@ __device__ __forceinline__ bool body_page_tables(const KTask& t, int vb, unsigne
 // args: k, v, tok, [fork], k_cache, v_cache.  cache[slot / ps][head][slot % ps][:] = k[token][head][:], rounded to the cache's type
 // (to nearest even: the type is the caller's choice); tokens without a slot are passed over.  A fork (src, dst, n) copies the
 // first n tokens of a page; new tokens are written behind them, and src's first n are written by nobody, so the order of the
-// two does not matter and a second run gives the same.  Bound by HBM: every byte is moved once, 16 at a time, eight loads of a thread under
-// way: 8192 tokens of 8 heads of 128 into bf16, 100 MB, 21.0 us (0.74 of the measured copy rate), 128 beams with 40 forks 4.1.
+// two does not matter and a second run gives the same.  Every byte is moved once, 16 at a time, eight loads of a thread under
+// way: 8192 tokens of 8 heads of 128 into bf16, 100 MB, 21.0 us (0.74 of the measured copy rate: 2048 blocks of one batch of loads each, five
+// to an SM, are 2.8 rounds, each with a start and an end in which little moves), 128 beams with 40 forks 4.1.
 constexpr int kAppendPerBlock = 4 * kThreads * 4;       // fp32 values of k, and of v
 __host__ inline int append_token_blocks(const PagedP& p) {
     return (int)(((long long)p.tokens * p.kvh * p.d + kAppendPerBlock - 1) / kAppendPerBlock);
