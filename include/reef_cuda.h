@@ -129,8 +129,10 @@ REEF_API reef_status reef_kernel_cost(const char* name, double* flops, double* b
 
 /* Binds a kernel handle to its device pointers ahead of the first launch (no reference counterpart): builds
  * the TMA tensor maps of tensor-core kernels and does every one-time allocation or attribute call, so
- * that the first reef_launch can already be part of a CUDA-graph capture.  Optional: a launch prepares
- * lazily when the pointers it is given differ from the prepared ones. */
+ * that the first reef_launch can already be part of a CUDA-graph capture.  Once on a device it is needed ahead of
+ * kernels that take more than 48 KB of shared memory (dense, fp32 convolution, staged attention, page tables, paged
+ * attention); beyond that it is optional: a launch prepares lazily when the pointers it is given differ from the
+ * prepared ones.  A device that cannot be prepared is reported, and the next call tries again. */
 REEF_API reef_status reef_kernel_prepare(reef_kernel_t k, void** args);
 
 /* Least size in bytes of the buffer behind each of the kernel's positional arguments (n >= its argument count).
